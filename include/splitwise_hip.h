@@ -39,7 +39,9 @@ typedef enum sw_dtype {
   SW_F32 = 0,
   SW_F16 = 1,
   SW_BF16 = 2,
-  SW_FP8_E5M2 = 3          /* unscaled e5m2 stored as uint8 (kv_cache_dtype "fp8_e5m2") */
+  SW_FP8_E5M2 = 3,         /* unscaled e5m2 stored as uint8 (kv_cache_dtype "fp8_e5m2") */
+  SW_I8_SCALED = 4,        /* int8 / e4m3 codes with a scale for each (block, kv head): only */
+  SW_E4M3_SCALED = 5       /* the *_scaled entry points take these two                       */
 } sw_dtype;
 
 const char* sw_last_error(void);
@@ -53,8 +55,10 @@ const char* sw_last_error(void);
  * 7: sw_context_attention_split, sw_context_attention_split_parts, sw_context_attention_split_workspace_bytes
  *    added.
  * 8: sw_prefill_attention_and_cache added.
- * 9: sw_paged_attention_and_cache added. */
-#define SW_ABI_VERSION 9
+ * 9: sw_paged_attention_and_cache added.
+ * 10: sw_reshape_and_cache_scaled, sw_gather_cache_scaled, sw_paged_attention_scaled, sw_context_attention_scaled,
+ *     sw_scaled_attention_parts, sw_scaled_attention_workspace_bytes added. */
+#define SW_ABI_VERSION 10
 int sw_abi_version(void);
 
 /* csrc/cuda_utils_kernels.cu:16-35 get_max_shared_memory_per_block_device_attribute:
@@ -415,6 +419,67 @@ int sw_context_attention_split(void* out, const void* query, const void* key, co
                                int64_t out_stride, int64_t kv_block_stride, int64_t kv_head_stride,
                                int sliding_window, int act_dtype, int64_t total_rows, int num_parts,
                                void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ------------------------------------------- an 8-bit cache with a scale for each (block, kv head)
+ * No counterpart in the reference, whose 8-bit cache is unscaled e5m2.  Codes are one byte, int8 in -127 .. 127
+ * (SW_I8_SCALED) or e4m3 (SW_E4M3_SCALED), and stand for code * scale:
+ *   key_cache      [num_blocks, kv_heads, head_size/16, block_size, 16]       key_scales    fp32 [num_blocks, kv_heads]
+ *   value_cache    [num_blocks, kv_heads, head_size, block_size]              value_scales  fp32 [num_blocks, kv_heads]
+ * all contiguous, the caches on 16 bytes.  head_size 64, 80, 96, 112, 128 or 256, block_size 8, 16 or 32.  A block table's
+ * entry outside 0 .. num_blocks - 1 is a block that does not exist: its tokens are read as zeros, and no row attends to them. */
+
+/* Quantises [num_tokens, num_heads, head_size] keys and values (SW_F32 / SW_F16 / SW_BF16, rows on 16 bytes) into the
+ * slots.  For the tokens of a call that go to one (block, head): scale = max(the block's, max |x| / 127 or / 448 over finite x;
+ * magnitudes below 2^-100 count as 0), code = x / scale to the nearest, infinities the largest code, NaN 0; codes that are there are
+ * rescaled.  A token for a block's first slot starts the block over: what it held, scales too, goes, and its other slots are zeros
+ * unless the call writes them.  Slots outside 0 .. num_blocks * block_size - 1 are padding.  Tokens of one block may stand anywhere
+ * in the list.  Of several tokens for one slot the last one stays, unless one run of neighbours in the list fills the whole block
+ * in order: then which one does is not specified. */
+int sw_reshape_and_cache_scaled(const void* key, const void* value, void* key_cache, void* value_cache,
+                                float* key_scales, float* value_scales, const int64_t* slot_mapping, int num_tokens,
+                                int num_heads, int head_size, int block_size, int64_t num_blocks, int64_t key_stride,
+                                int64_t value_stride, int act_dtype, int cache_dtype, void* stream);
+
+/* Reads seq_lens[i] tokens of block_tables row i back into rows seq_starts[i] .. of key and value ([num_rows, num_heads,
+ * head_size], SW_F32 / SW_F16 / SW_BF16, rows on 16 bytes): code * scale, rounded once.  Tokens from max_seq_len (rounded up to whole
+ * blocks) or from max_blocks_per_seq blocks on are not read, rows from num_rows on and those of no sequence not written. */
+int sw_gather_cache_scaled(void* key, void* value, const void* key_cache, const void* value_cache,
+                           const float* key_scales, const float* value_scales, const int32_t* block_tables,
+                           const int32_t* seq_starts, const int32_t* seq_lens, int num_seqs, int max_seq_len,
+                           int64_t num_rows, int num_heads, int head_size, int block_size, int64_t num_blocks,
+                           int max_blocks_per_seq, int64_t table_stride, int64_t key_stride, int64_t value_stride,
+                           int act_dtype, int cache_dtype, void* stream);
+
+/* Attention of one new token a sequence (query / out [num_seqs, num_heads, head_size], SW_F16 / SW_BF16, rows on 16 bytes), the
+ * last of its context_lens[i], over the cache.  alibi_slopes fp32 [num_heads] or NULL.  A sequence of no tokens gives zeros.
+ * num_parts: workgroups that share a context, 1 or more; above 1 they leave their sums in the workspace
+ * (sw_scaled_attention_workspace_bytes, 16-byte aligned, any contents) and a second kernel joins them. */
+int sw_paged_attention_scaled(void* out, const void* query, const void* key_cache, const void* value_cache,
+                              const float* key_scales, const float* value_scales, int num_seqs, int num_heads,
+                              int num_kv_heads, int head_size, float scale, const int32_t* block_tables,
+                              const int32_t* context_lens, int block_size, int64_t num_blocks, int max_context_len,
+                              int max_blocks_per_seq, int64_t table_stride, const float* alibi_slopes, int64_t q_stride,
+                              int64_t out_stride, int act_dtype, int cache_dtype, int num_parts, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+
+/* Attention of the last new_lens[i] tokens of a sequence's seq_lens[i], which are all in the cache, over the cache: row
+ * seq_starts[i] + j of query / out ([num_rows, num_heads, head_size]) is token seq_lens[i] - new_lens[i] + j and sees the tokens up to
+ * itself, the last sliding_window of them if that is above 0.  Rows of no sequence are not written.  Otherwise as
+ * sw_paged_attention_scaled; max_new_len bounds new_lens, of which no more are done. */
+int sw_context_attention_scaled(void* out, const void* query, const void* key_cache, const void* value_cache,
+                                const float* key_scales, const float* value_scales, int num_seqs, int64_t num_rows,
+                                int num_heads, int num_kv_heads, int head_size, float scale,
+                                const int32_t* block_tables, const int32_t* seq_starts, const int32_t* new_lens,
+                                const int32_t* seq_lens, int block_size, int64_t num_blocks, int max_new_len,
+                                int max_context_len, int max_blocks_per_seq, int64_t table_stride,
+                                const float* alibi_slopes, int sliding_window, int64_t q_stride, int64_t out_stride,
+                                int act_dtype, int cache_dtype, int num_parts, void* workspace,
+                                int64_t workspace_bytes, void* stream);
+
+/* The number of parts for a launch of that shape, and the bytes of workspace for it (0 for one part). */
+int sw_scaled_attention_parts(int num_seqs, int max_new_len, int num_heads, int num_kv_heads, int head_size,
+                              int max_context_len);
+int64_t sw_scaled_attention_workspace_bytes(int num_parts, int64_t num_rows, int num_heads, int head_size);
 
 /* ------------------------------------------------------- all-reduce by direct peer reads
  * Replaces csrc/custom_all_reduce.cu:12-148 / custom_all_reduce.cuh:341-548 (init_custom_ar,

@@ -1,0 +1,326 @@
+// Attention of few rows over the 8-bit cache with one scale for each (block, kv head) (included by scaled_decode_*.hip).
+//
+//     o = sum_t p_t sv_t v_t / sum_t p_t,    p_t = exp(scale * sk_t q.k_t + slope * (t - position) - m)
+// over the codes k_t, v_t with the scales sk, sv of their blocks.  Bound by the cache's bytes: one per element, read once for up to 16
+// rows (query heads of the kv head, and new tokens), so the products run on the matrix cores however few rows there are, and nothing
+// but the codes is fetched for an element.
+//
+// A wave takes 64 tokens at a time, four runs of 16, and forms
+//     S [16 tokens x 16 rows]  = K tile . Q^T             (v_mfma_f32_16x16x32_f16, four tiles)
+//     O^T [16 dims x 16 rows] += V^T tile . P^T
+// Codes are widened to halves exactly (integers up to 127; e4m3), after the load, in registers: 16 bytes of a lane are 16 dims of a
+// key or 16 tokens of a dim's values, as the caches lie.  Both products may take their contraction in any order that their two operands
+// share, and S's tokens any place among its rows, so that nothing changes hands between them:
+//     K tile j, row r            <->  token 4 j + (r & 3) of run r >> 2
+//     Q.K  slot (kq, e) of step 2 m + h  <->  dim 64 m + 16 kq + 8 h + e
+//     S tile j of lane (kq, row), i      <->  token 4 j + i of run kq: 16 weights, which are
+//     P.V  slot (kq, e) of step h        <->  token 8 h + e of run kq
+// Scales are a factor of the score and of the weight, both fp32.  The weights go to the second product as halves (an error of 2^-12, under
+// what bf16's 2^-9 or f16's 2^-12 rounding of the result leaves), relative to the largest value scale met so far, which goes into the
+// sums as the maximum does: p sv / r is at most 1 whatever the scales are.  bf16 queries go into halves by a power of two for each row
+// that brings their largest to 2^14 .. 2^15, which goes into the row's scale.
+#pragma once
+
+#include "scaled_attention.cuh"
+
+namespace sw {
+
+// NW waves take the groups of 64 tokens of one (sequence, kv head, tile of 16 rows, part) in turn and join at the end.
+// EXACT: head_size == HEAD; else it is a smaller multiple of 16 (dims behind it count as zeros).
+template <bool E4M3, int HEAD, bool EXACT, int BS, int NW>
+__global__ void __launch_bounds__(NW * 64) scaled_decode_kernel(const ScAttention a) {
+  using C = ScCode<E4M3>;
+  constexpr int KM = HEAD / 64, DT = HEAD / 16;
+  constexpr int PB = BS == 8 ? 2 : 1;                        // blocks of a run of 16 tokens
+  extern __shared__ __attribute__((aligned(16))) float smem[];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, kq = lane >> 4;
+  const int seq = blockIdx.y, part = blockIdx.z;
+  const int kv_head = blockIdx.x / a.tiles, tile = blockIdx.x - kv_head * a.tiles;
+  const ScSequence s = sc_sequence<BS>(a, seq);
+  const int rows = s.fresh * a.group;
+  if (tile * 16 >= rows) return;
+  const int head_size = EXACT ? HEAD : a.head_size;
+
+  // this lane's row: a new token and a query head of the kv head
+  const int my = tile * 16 + r;
+  const bool real = my < rows;
+  const int row_tok = real ? my / a.group : 0, head = kv_head * a.group + (real ? my - row_tok * a.group : 0);
+  const int pos = s.first + row_tok;                 // sees tokens up to its own
+  // what the tile's rows see, of which this part
+  const int last_tok = min(rows - 1, tile * 16 + 15) / a.group;
+  const int pos_low = s.first + tile * 16 / a.group, pos_high = s.first + last_tok;
+  const int seen_from = sc_seen_from(a, pos_low);            // a multiple of 64, as the parts' borders are
+  const int begin = max(part * a.part_tokens, seen_from), end = sc_part_end(a, s, part, pos_high);
+  if (a.partial && begin >= end) return;                     // (the join knows)
+  // rows that all see a token: from here on the mask is to be looked at
+  const int all_see = pos_low + 1, none_hidden = a.window > 0 ? pos_high - a.window + 1 : 0;
+
+  sc_u32x4 qf[KM][2];
+  float row_scale = a.scale2;
+  {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(a.query) + (s.row0 + row_tok) * a.q_stride + (int64_t)head * head_size;
+    float largest = 0.f;
+#pragma unroll
+    for (int m = 0; m < KM; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int d = 64 * m + 16 * kq + 8 * h;
+        qf[m][h] = real && (EXACT || d < head_size) ? *reinterpret_cast<const sc_u32x4*>(q + d) : sc_u32x4{0u, 0u, 0u, 0u};
+        if (a.bf16) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            largest = fmaxf(largest, fmaxf(fabsf(bf16_bits_to_float((uint16_t)(qf[m][h][w] & 0xffffu))),
+                                           fabsf(bf16_bits_to_float((uint16_t)(qf[m][h][w] >> 16)))));
+        }
+      }
+    if (a.bf16) {
+      largest = fmaxf(largest, __shfl_xor(largest, 16, 64));
+      largest = fmaxf(largest, __shfl_xor(largest, 32, 64));
+      float up = 1.f;
+      if (largest > 0.f && largest < INFINITY) {
+        const int e = min(15 - (int)__builtin_amdgcn_frexp_expf(largest), 126);
+        up = ldexpf(1.f, e);
+        row_scale = ldexpf(row_scale, -e);
+      }
+#pragma unroll
+      for (int m = 0; m < KM; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            qf[m][h][w] = sc_pack_f16(bf16_bits_to_float((uint16_t)(qf[m][h][w] & 0xffffu)) * up,
+                                      bf16_bits_to_float((uint16_t)(qf[m][h][w] >> 16)) * up);
+    }
+  }
+  const float slope = a.slopes ? a.slopes[head] * 1.44269504088896340736f : 0.f;
+
+  const int64_t head_bytes = (int64_t)head_size * BS;
+  const int32_t* table = a.tables + (int64_t)seq * a.table_stride;
+
+  float m_run = -INFINITY, l_run = 0.f, r_run = 0.f;
+  sc_f32x4 acc[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) acc[dt] = sc_f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const int first_group = begin >> 6, groups = (end + 63) >> 6;
+  for (int g = first_group + wave; g < groups; g += NW) {
+    const int tok0 = g << 6;
+    // blocks of the run whose keys this lane loads (r >> 2) and of the one whose values it loads and scores it gets (kq)
+    int kb[PB], vb[PB];
+    uint32_t good = 0xffffu;                                  // tokens of run kq that there are
+    sc_u32x4 kraw[4][KM], vraw[DT];
+    float ks[PB], vs[PB];
+    const int last_block = (s.len - 1) / BS;
+#pragma unroll
+    for (int b = 0; b < PB; ++b) {
+      kb[b] = table[min((tok0 + 16 * (r >> 2) + 8 * b) / BS, last_block)];
+      vb[b] = table[min((tok0 + 16 * kq + 8 * b) / BS, last_block)];
+      if (kb[b] < 0 || kb[b] >= a.num_blocks) kb[b] = 0;
+      if (vb[b] < 0 || vb[b] >= a.num_blocks) {
+        vb[b] = 0;
+        good &= PB == 1 ? 0u : b == 0 ? 0xff00u : 0x00ffu;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int o = 4 * j + (r & 3);                          // token of the run
+      const int b = PB == 2 ? j >> 1 : 0;
+      const int off = BS == 8 ? o & 7 : BS == 16 ? o : ((r >> 2) & 1) * 16 + o;
+      const uint8_t* p = a.key_cache + ((int64_t)kb[b] * a.kv_heads + kv_head) * head_bytes + off * 16;
+#pragma unroll
+      for (int m = 0; m < KM; ++m)
+        kraw[j][m] = EXACT || 64 * m + 16 * kq < head_size ? *reinterpret_cast<const sc_u32x4*>(p + (4 * m + kq) * (BS * 16))
+                                                           : sc_u32x4{0u, 0u, 0u, 0u};
+    }
+#pragma unroll
+    for (int b = 0; b < PB; ++b) {
+      ks[b] = a.key_scales[(int64_t)vb[b] * a.kv_heads + kv_head];
+      vs[b] = a.value_scales[(int64_t)vb[b] * a.kv_heads + kv_head];
+    }
+    {
+      const uint8_t* p[PB];
+#pragma unroll
+      for (int b = 0; b < PB; ++b)
+        p[b] = a.value_cache + ((int64_t)vb[b] * a.kv_heads + kv_head) * head_bytes + r * BS + (BS == 32 ? (kq & 1) * 16 : 0);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        if (!EXACT && 16 * dt >= head_size) {
+          vraw[dt] = sc_u32x4{0u, 0u, 0u, 0u};
+        } else if constexpr (PB == 2) {
+          vraw[dt] = sc_join(*reinterpret_cast<const sc_u32x2*>(p[0] + 16 * dt * BS), *reinterpret_cast<const sc_u32x2*>(p[1] + 16 * dt * BS));
+        } else {
+          vraw[dt] = *reinterpret_cast<const sc_u32x4*>(p[0] + 16 * dt * BS);
+        }
+      }
+    }
+
+    // ---- scores: lane (kq, row r), tokens tok0 + 16 kq + 4 j + i
+    sc_f32x4 x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = sc_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int m = 0; m < KM; ++m)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j] = sc_mfma(sc_join(C::widen(kraw[j][m][0]), C::widen(kraw[j][m][1])), qf[m][0], x[j]);
+        x[j] = sc_mfma(sc_join(C::widen(kraw[j][m][2]), C::widen(kraw[j][m][3])), qf[m][1], x[j]);
+      }
+    const int run0 = tok0 + 16 * kq;
+    const int left = end - run0;
+    good &= left >= 16 ? 0xffffu : left <= 0 ? 0u : (1u << left) - 1u;
+    // (wave-uniform) all 64 tokens are there and every row sees all of them
+    const bool masked = tok0 + 64 > all_see || tok0 < none_hidden || __any(good != 0xffffu);
+    float gmax = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float f = row_scale * ks[PB == 2 ? j >> 1 : 0];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = run0 + 4 * j + i;
+        float v = x[j][i] * f;
+        if (a.slopes) v += slope * (float)(t - pos);
+        if (masked) {
+          const bool see = (good >> (4 * j + i) & 1u) && t <= pos && (a.window <= 0 || t > pos - a.window);
+          v = see ? v : -INFINITY;
+        }
+        x[j][i] = v;
+        gmax = fmaxf(gmax, v);
+      }
+    }
+    float smax = 0.f;
+#pragma unroll
+    for (int b = 0; b < PB; ++b) {
+      if (masked && (PB == 1 ? good == 0 : (good >> (8 * b) & 0xffu) == 0)) vs[b] = 0.f;
+      smax = fmaxf(smax, vs[b]);
+    }
+    gmax = fmaxf(gmax, __shfl_xor(gmax, 16, 64));
+    gmax = fmaxf(gmax, __shfl_xor(gmax, 32, 64));
+    smax = fmaxf(smax, __shfl_xor(smax, 16, 64));
+    smax = fmaxf(smax, __shfl_xor(smax, 32, 64));
+    const float m_new = fmaxf(m_run, gmax), base = sc_base(m_new);
+    const float r_new = fmaxf(r_run, smax), r_inv = r_new > 0.f ? 1.f / r_new : 0.f;
+    const float alpha = __builtin_amdgcn_exp2f(m_run - base);
+    m_run = m_new;
+    const float shrink = alpha * (r_run * r_inv);
+    r_run = r_new;
+
+    // ---- weights: their sum, and as the second product takes them
+    sc_u32x4 pf[2];
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float f = vs[PB == 2 ? j >> 1 : 0] * r_inv;
+      float p[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(x[j][i] - base);
+        sum += p[i];
+      }
+      pf[j >> 1][2 * (j & 1)] = sc_pack_f16(p[0] * f, p[1] * f);
+      pf[j >> 1][2 * (j & 1) + 1] = sc_pack_f16(p[2] * f, p[3] * f);
+    }
+    l_run = l_run * alpha + sum;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[dt] *= shrink;
+
+    // ---- values.  Slots that hold no token may hold anything, an e4m3 NaN included, and 0 x NaN is NaN: cleared.
+    if (E4M3 && masked) {
+      sc_u32x4 keep;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t some = good >> (4 * w) & 15u;
+        keep[w] = (some & 1u ? 0xffu : 0u) | (some & 2u ? 0xff00u : 0u) | (some & 4u ? 0xff0000u : 0u) | (some & 8u ? 0xff000000u : 0u);
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) vraw[dt] &= keep;
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) {
+      acc[dt] = sc_mfma(sc_join(C::widen(vraw[dt][0]), C::widen(vraw[dt][1])), pf[0], acc[dt]);
+      acc[dt] = sc_mfma(sc_join(C::widen(vraw[dt][2]), C::widen(vraw[dt][3])), pf[1], acc[dt]);
+    }
+  }
+
+  // ---- the waves join: a common maximum, then pairs of waves by halves
+  l_run += __shfl_xor(l_run, 16, 64);
+  l_run += __shfl_xor(l_run, 32, 64);
+  float* stat = smem;                                         // [NW][2][16]
+  float* pass = smem + NW * 32;                               // [NW / 2][DT][64 lanes][4]
+  if (kq == 0) {
+    stat[wave * 32 + r] = m_run;
+    stat[wave * 32 + 16 + r] = l_run;
+  }
+  __syncthreads();
+  float m_all = -INFINITY, l_all = 0.f;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) m_all = fmaxf(m_all, stat[w * 32 + r]);
+  const float base = sc_base(m_all);
+#pragma unroll
+  for (int w = 0; w < NW; ++w) l_all += stat[w * 32 + 16 + r] * __builtin_amdgcn_exp2f(stat[w * 32 + r] - base);
+  const float mine = __builtin_amdgcn_exp2f(m_run - base) * r_run;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) acc[dt] *= mine;
+#pragma unroll
+  for (int half = NW / 2; half >= 1; half >>= 1) {
+    if (wave >= half && wave < 2 * half) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<sc_f32x4*>(pass + (((wave - half) * DT + dt) * 64 + lane) * 4) = acc[dt];
+    }
+    __syncthreads();
+    if (wave < half) {
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) acc[dt] += *reinterpret_cast<const sc_f32x4*>(pass + ((wave * DT + dt) * 64 + lane) * 4);
+    }
+    __syncthreads();
+  }
+  if (wave != 0 || !real) return;
+  if (a.partial) {
+    float* to = a.partial + (((s.row0 + row_tok) * a.heads + head) * a.parts + part) * (head_size + 4);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+      if (EXACT || 16 * dt < head_size) *reinterpret_cast<sc_f32x4*>(to + 16 * dt + 4 * kq) = acc[dt];
+    if (kq == 0) {
+      to[head_size] = m_all;
+      to[head_size + 1] = l_all;
+    }
+    return;
+  }
+  const float inv = l_all > 0.f ? 1.f / l_all : l_all != l_all ? l_all : 0.f;   // a row that sees nothing gives zeros
+  uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (s.row0 + row_tok) * a.out_stride + (int64_t)head * head_size;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+    if (EXACT || 16 * dt < head_size)
+      *reinterpret_cast<sc_u32x2*>(out + 16 * dt + 4 * kq) =
+          sc_u32x2{sc_pack16(acc[dt][0] * inv, acc[dt][1] * inv, a.bf16), sc_pack16(acc[dt][2] * inv, acc[dt][3] * inv, a.bf16)};
+}
+
+template <bool E4M3, int HEAD, bool EXACT, int BS, int NW>
+int sc_launch_decode(const ScAttention& a, int num_seqs, hipStream_t stream) {
+  const int lds = (NW * 32 + (NW / 2) * (HEAD / 16) * 256) * 4;
+  static_assert((NW * 32 + (NW / 2) * (HEAD / 16) * 256) * 4 <= 64 * 1024, "the waves' sums must fit a launch's plain LDS");
+  scaled_decode_kernel<E4M3, HEAD, EXACT, BS, NW><<<dim3(a.kv_heads * a.tiles, num_seqs, a.parts), NW * 64, lds, stream>>>(a);
+  SW_CHECK_LAUNCH();
+  return SW_OK;
+}
+
+template <bool E4M3, int NW>
+int sc_decode_by_size(const ScAttention& a, int block_size, int num_seqs, hipStream_t stream) {
+  auto by_block = [&](auto head, auto exact) {
+    constexpr int H = decltype(head)::value;
+    constexpr bool X = decltype(exact)::value;
+    return block_size == 8    ? sc_launch_decode<E4M3, H, X, 8, NW>(a, num_seqs, stream)
+           : block_size == 16 ? sc_launch_decode<E4M3, H, X, 16, NW>(a, num_seqs, stream)
+                              : sc_launch_decode<E4M3, H, X, 32, NW>(a, num_seqs, stream);
+  };
+  switch (a.head_size) {
+    case 64: return by_block(std::integral_constant<int, 64>{}, std::true_type{});
+    case 128: return by_block(std::integral_constant<int, 128>{}, std::true_type{});
+    case 256: return by_block(std::integral_constant<int, 256>{}, std::true_type{});
+    default: return by_block(std::integral_constant<int, 128>{}, std::false_type{});
+  }
+}
+
+}  // namespace sw

@@ -1,0 +1,7 @@
+#include "scaled_decode.cuh"
+
+namespace sw {
+int sc_decode_e4m3(const ScAttention& a, int block_size, int num_seqs, hipStream_t stream) {
+  return sc_decode_by_size<true, 4>(a, block_size, num_seqs, stream);
+}
+}  // namespace sw

@@ -1,0 +1,7 @@
+#include "scaled_decode.cuh"
+
+namespace sw {
+int sc_decode_i8(const ScAttention& a, int block_size, int num_seqs, hipStream_t stream) {
+  return sc_decode_by_size<false, 4>(a, block_size, num_seqs, stream);
+}
+}  // namespace sw

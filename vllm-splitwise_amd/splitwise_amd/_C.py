@@ -24,7 +24,7 @@ from ._native import bind_library, step_ops as _native
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libsplitwise_hip.so")
 
-SW_F32, SW_F16, SW_BF16, SW_FP8_E5M2 = 0, 1, 2, 3
+SW_F32, SW_F16, SW_BF16, SW_FP8_E5M2, SW_I8_SCALED, SW_E4M3_SCALED = 0, 1, 2, 3, 4, 5
 _TORCH_TO_SW = {torch.float32: SW_F32, torch.float16: SW_F16, torch.bfloat16: SW_BF16}
 
 _c_void_p = ctypes.c_void_p
@@ -81,6 +81,16 @@ _SIGNATURES = {
                                   + [_c_i64] * 6 + [_c_int, _c_int, _c_i64, _c_int, _c_void_p, _c_i64, _c_void_p],
     "sw_context_attention_split_parts": [_c_int] * 6,
     "sw_context_attention_split_workspace_bytes": [_c_int, _c_i64, _c_int, _c_int],
+    "sw_reshape_and_cache_scaled": [_c_void_p] * 7 + [_c_int] * 4 + [_c_i64] * 3 + [_c_int] * 2 + [_c_void_p],
+    "sw_gather_cache_scaled": [_c_void_p] * 9 + [_c_int] * 2 + [_c_i64] + [_c_int] * 3 + [_c_i64, _c_int] + [_c_i64] * 3
+                              + [_c_int] * 2 + [_c_void_p],
+    "sw_paged_attention_scaled": [_c_void_p] * 6 + [_c_int] * 4 + [_c_float] + [_c_void_p] * 2 + [_c_int, _c_i64, _c_int, _c_int, _c_i64]
+                                 + [_c_void_p] + [_c_i64] * 2 + [_c_int] * 3 + [_c_void_p, _c_i64, _c_void_p],
+    "sw_context_attention_scaled": [_c_void_p] * 6 + [_c_int, _c_i64] + [_c_int] * 3 + [_c_float] + [_c_void_p] * 4
+                                   + [_c_int, _c_i64] + [_c_int] * 3 + [_c_i64, _c_void_p, _c_int] + [_c_i64] * 2 + [_c_int] * 3
+                                   + [_c_void_p, _c_i64, _c_void_p],
+    "sw_scaled_attention_parts": [_c_int] * 6,
+    "sw_scaled_attention_workspace_bytes": [_c_int, _c_i64, _c_int, _c_int],
     "sw_custom_ar_signal_bytes": [],
     "sw_custom_ar_init": [ctypes.POINTER(_c_void_p), _c_int, _c_int, _c_i64, _c_i64, _c_i64, _c_i64,
                           ctypes.POINTER(_c_void_p)],
@@ -102,7 +112,8 @@ _SIGNATURES = {
 }
 _RESTYPES = {"sw_quant_gemm_workspace_bytes": _c_i64, "sw_custom_ar_signal_bytes": _c_i64,
              "sw_paged_attention_v2_static_max_bytes": _c_i64,
-             "sw_context_attention_split_workspace_bytes": _c_i64}     # everything else returns an int status
+             "sw_context_attention_split_workspace_bytes": _c_i64,
+             "sw_scaled_attention_workspace_bytes": _c_i64}     # everything else returns an int status
 
 _lib = None
 
@@ -111,7 +122,7 @@ def library_path() -> str:
     return _LIB_PATH
 
 
-ABI_VERSION = 9                # SW_ABI_VERSION of include/splitwise_hip.h this binding was written against
+ABI_VERSION = 10               # SW_ABI_VERSION of include/splitwise_hip.h this binding was written against
 
 
 def load_library() -> ctypes.CDLL:
@@ -552,6 +563,186 @@ def context_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: 
             _check(lib.sw_context_attention(*args, _stream(q)))
 
 
+# ---------------------------------------------- the 8-bit cache with a scale for each (block, kv head)
+_SCALED = {"int8": SW_I8_SCALED, "fp8_e4m3": SW_E4M3_SCALED}
+
+
+def _scaled_caches(name: str, kv_cache_dtype: str, like: torch.Tensor, head_size: int, num_kv_heads: int, key_cache: torch.Tensor,
+                   value_cache: torch.Tensor, key_scales: torch.Tensor, value_scales: torch.Tensor, *others: torch.Tensor) -> int:
+    """The cache type's number; raises where the tensors are not such a cache (and such scales) on ``like``'s device.  Shapes: the
+    kernels index by them, so they are looked at one by one."""
+    cache = _SCALED.get(kv_cache_dtype)
+    if cache is None:
+        raise RuntimeError(f"{name}: Unsupported data type of kv cache: {kv_cache_dtype} (one of {', '.join(_SCALED)})")
+    if key_cache.dtype != torch.uint8 or value_cache.dtype != torch.uint8:
+        raise RuntimeError(f"{name}: the caches hold their codes as uint8")
+    if key_scales.dtype != torch.float32 or value_scales.dtype != torch.float32:
+        raise RuntimeError(f"{name}: scales must be float32")
+    if value_cache.dim() != 4:
+        raise RuntimeError(f"{name}: value cache [blocks, kv heads, head size, block size]")
+    blocks, heads, size, block = value_cache.shape
+    if heads != num_kv_heads or size != head_size or key_cache.shape != (blocks, heads, size // 16, block, 16):
+        raise RuntimeError(f"{name}: key cache [blocks, kv heads, head size / 16, block size, 16] and value cache [blocks, kv heads, "
+                           f"head size, block size] for {num_kv_heads} heads of {head_size}: got {tuple(key_cache.shape)}, "
+                           f"{tuple(value_cache.shape)}")
+    if key_scales.shape != (blocks, heads) or value_scales.shape != (blocks, heads):
+        raise RuntimeError(f"{name}: scales [blocks, kv heads]")
+    if not (key_cache.is_contiguous() and value_cache.is_contiguous() and key_scales.is_contiguous() and value_scales.is_contiguous()):
+        raise RuntimeError(f"{name}: caches and scales must be contiguous")
+    device = like.device
+    for t in (key_cache, value_cache, key_scales, value_scales) + others:
+        if t.device != device:
+            raise RuntimeError(f"{name}: all tensors must be on {device}")
+    if not like.is_cuda:
+        raise RuntimeError("splitwise_hip operators need tensors on a HIP device")
+    return cache
+
+
+def _scaled_rows(name: str, *tensors: torch.Tensor) -> None:
+    for t in tensors:
+        if t.dim() != 3 or t.shape != tensors[0].shape or t.dtype != tensors[0].dtype:
+            raise RuntimeError(f"{name}: [tokens, heads, head size] tensors of one shape and type")
+        if t.numel() and (t.stride(2) != 1 or t.stride(1) != t.shape[2]):
+            raise RuntimeError(f"{name}: heads must be contiguous")
+
+
+def _scaled_table(name: str, block_tables: torch.Tensor, *lengths: torch.Tensor) -> None:
+    for t in lengths:
+        if t.dtype != torch.int32 or t.shape != (block_tables.shape[0],) or not t.is_contiguous():
+            raise RuntimeError(f"{name}: starts and lengths must be contiguous int32, one for each row of the block tables")
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2:
+        raise RuntimeError(f"{name}: block_tables must be int32 [sequences, blocks]")
+    if block_tables.numel() and block_tables.stride(1) != 1:
+        raise RuntimeError(f"{name}: block_tables rows must be contiguous")
+
+
+def reshape_and_cache_scaled(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                             key_scales: torch.Tensor, value_scales: torch.Tensor, slot_mapping: torch.Tensor,
+                             kv_cache_dtype: str) -> None:
+    """``reshape_and_cache`` into a cache held in 8 bits (``kv_cache_dtype`` "int8" or "fp8_e4m3", uint8 tensors) with one fp32 scale
+    for each (block, kv head): key / value [T, KVH, D] in fp16, bf16 or fp32, caches [blocks, KVH, D/16, bs, 16] and
+    [blocks, KVH, D, bs], scales [blocks, KVH].
+
+    A block's scale is its largest finite magnitude over 127 (448).  It grows when a call brings a larger one, and what the block held
+    is rescaled; it starts over with the token for the block's first slot, whose other slots become zeros unless the call writes them.
+    Infinities go to the largest code, NaN to 0.  Slots outside the cache (negative: padding) are skipped.  A block's
+    tokens may stand anywhere in the list, and of several for one slot the last one stays (unless neighbours in the list fill the whole
+    block in order: then which one does is not specified)."""
+    name = "reshape_and_cache_scaled"
+    _scaled_rows(name, key, value)
+    if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (key.shape[0],) or not slot_mapping.is_contiguous():
+        raise RuntimeError(f"{name}: slot_mapping must be contiguous int64, one for each token")
+    cache = _scaled_caches(name, kv_cache_dtype, key, key.shape[2], key.shape[1], key_cache, value_cache, key_scales, value_scales,
+                           value, slot_mapping)
+    with _on_device_of(key):
+        _check(load_library().sw_reshape_and_cache_scaled(
+            key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
+            value_scales.data_ptr(), slot_mapping.data_ptr(), key.shape[0], key.shape[1], key.shape[2], value_cache.shape[3],
+            value_cache.shape[0], key.stride(0), value.stride(0), _act_dtype(key), cache, _stream(key)))
+
+
+def gather_cache_scaled(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                        key_scales: torch.Tensor, value_scales: torch.Tensor, block_tables: torch.Tensor, seq_starts: torch.Tensor,
+                        seq_lens: torch.Tensor, max_seq_len: int, kv_cache_dtype: str) -> None:
+    """Reads a cache written by ``reshape_and_cache_scaled`` back: the first ``seq_lens[i]`` tokens of block table i into rows
+    ``seq_starts[i]`` .. of key and value [rows, KVH, D] (fp16, bf16 or fp32), code * scale rounded once.  ``max_seq_len`` bounds the
+    lengths (rounded up to whole blocks, no more is read).  Rows of no sequence stay as they are, rows behind the tensors' end are left out,
+    and tokens of blocks that do not exist are zeros.  Sequences must not share rows."""
+    name = "gather_cache_scaled"
+    _scaled_rows(name, key, value)
+    _scaled_table(name, block_tables, seq_starts, seq_lens)
+    cache = _scaled_caches(name, kv_cache_dtype, key, key.shape[2], key.shape[1], key_cache, value_cache, key_scales, value_scales,
+                           value, block_tables, seq_starts, seq_lens)
+    with _on_device_of(key):
+        _check(load_library().sw_gather_cache_scaled(
+            key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
+            value_scales.data_ptr(), block_tables.data_ptr(), seq_starts.data_ptr(), seq_lens.data_ptr(), seq_lens.shape[0],
+            int(max_seq_len), key.shape[0], key.shape[1], key.shape[2], value_cache.shape[3], value_cache.shape[0],
+            block_tables.shape[1], block_tables.stride(0), key.stride(0), value.stride(0), _act_dtype(key), cache, _stream(key)))
+
+
+def _scaled_attention(name: str, out, query, key_cache, value_cache, key_scales, value_scales, num_kv_heads, alibi_slopes,
+                      kv_cache_dtype, block_tables, *lengths):
+    """The checks of both; (cache type's number, slopes on the device)."""
+    _scaled_rows(name, query, out)
+    if alibi_slopes is not None:
+        if alibi_slopes.dtype != torch.float32 or alibi_slopes.shape != (query.shape[1],):
+            raise RuntimeError(f"{name}: alibi_slopes must be float32, one for each query head")
+        alibi_slopes = alibi_slopes.to(query.device).contiguous()
+    if query.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError(f"{name}: Unsupported data type: {query.dtype}")
+    _scaled_table(name, block_tables, *lengths)
+    cache = _scaled_caches(name, kv_cache_dtype, query, query.shape[2], num_kv_heads, key_cache, value_cache, key_scales, value_scales,
+                           out, block_tables, *lengths)
+    return cache, alibi_slopes
+
+
+def _scaled_workspace(lib, num_parts: Optional[int], num_seqs: int, max_new_len: int, num_kv_heads: int, max_context_len: int,
+                      query: torch.Tensor):
+    """(parts, workspace or None, its bytes): from torch's caching allocator, so that a captured call has its own."""
+    rows, heads, size = query.shape
+    if num_parts is None:
+        num_parts = lib.sw_scaled_attention_parts(num_seqs, max_new_len, heads, num_kv_heads, size, max_context_len)
+    nbytes = int(lib.sw_scaled_attention_workspace_bytes(num_parts, rows, heads, size))
+    return num_parts, torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None, nbytes
+
+
+def paged_attention_scaled(out: torch.Tensor, query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                           key_scales: torch.Tensor, value_scales: torch.Tensor, num_kv_heads: int, scale: float,
+                           block_tables: torch.Tensor, context_lens: torch.Tensor, block_size: int, max_context_len: int,
+                           alibi_slopes: Optional[torch.Tensor], kv_cache_dtype: str, num_parts: Optional[int] = None) -> None:
+    """``paged_attention_v1`` / ``_v2`` over a cache written by ``reshape_and_cache_scaled``: out / query [S, H, D] in fp16 or bf16, the
+    query of sequence i being the last of its ``context_lens[i]`` tokens.  A sequence of no tokens gives zeros, and so does one whose
+    blocks do not exist (table entries outside the cache).  ``num_parts``: workgroups that share a context; None lets the library
+    decide by the launch's shape and ``max_context_len``."""
+    name = "paged_attention_scaled"
+    if query.dim() == 3 and query.shape[0] != block_tables.shape[0]:
+        raise RuntimeError(f"{name}: one row of block_tables for each query")
+    if value_cache.dim() == 4 and value_cache.shape[3] != block_size:
+        raise RuntimeError(f"{name}: the cache has blocks of {value_cache.shape[3]} tokens, not {block_size}")
+    cache, alibi_slopes = _scaled_attention(name, out, query, key_cache, value_cache, key_scales, value_scales, num_kv_heads,
+                                            alibi_slopes, kv_cache_dtype, block_tables, context_lens)
+    num_seqs, num_heads, head_size = query.shape
+    lib = load_library()
+    with _on_device_of(query):
+        num_parts, workspace, nbytes = _scaled_workspace(lib, num_parts, num_seqs, 1, num_kv_heads, int(max_context_len), query)
+        _check(lib.sw_paged_attention_scaled(
+            out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
+            value_scales.data_ptr(), num_seqs, num_heads, num_kv_heads, head_size, float(scale), block_tables.data_ptr(),
+            context_lens.data_ptr(), block_size, value_cache.shape[0], int(max_context_len), block_tables.shape[1],
+            block_tables.stride(0), alibi_slopes.data_ptr() if alibi_slopes is not None else None, query.stride(0), out.stride(0),
+            _act_dtype(query), cache, num_parts, workspace.data_ptr() if nbytes else None, nbytes, _stream(query)))
+
+
+def context_attention_scaled(out: torch.Tensor, query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                             key_scales: torch.Tensor, value_scales: torch.Tensor, scale: float, block_tables: torch.Tensor,
+                             seq_starts: torch.Tensor, new_lens: torch.Tensor, seq_lens: torch.Tensor, max_new_len: int,
+                             max_context_len: int, alibi_slopes: Optional[torch.Tensor], kv_cache_dtype: str,
+                             sliding_window: Optional[int] = None, num_parts: Optional[int] = None) -> None:
+    """Attention of the last ``new_lens[i]`` of a sequence's ``seq_lens[i]`` tokens, all of which are in the cache (written by
+    ``reshape_and_cache_scaled``): prompts behind a cached prefix, chunks of a prompt, drafted tokens.  Row ``seq_starts[i] + j`` of
+    query and out [rows, H, D] (fp16 or bf16) is the sequence's token ``seq_lens[i] - new_lens[i] + j`` and sees the tokens up to itself,
+    with ``sliding_window`` the last that many.  ``max_new_len`` and ``max_context_len`` bound new_lens and seq_lens; new tokens beyond the
+    former are not computed.  Rows of no sequence stay as they are; sequences must not share rows."""
+    name = "context_attention_scaled"
+    num_kv_heads = value_cache.shape[1] if value_cache.dim() == 4 else 0
+    cache, alibi_slopes = _scaled_attention(name, out, query, key_cache, value_cache, key_scales, value_scales, num_kv_heads,
+                                            alibi_slopes, kv_cache_dtype, block_tables, seq_starts, new_lens, seq_lens)
+    rows, num_heads, head_size = query.shape
+    lib = load_library()
+    with _on_device_of(query):
+        num_parts, workspace, nbytes = _scaled_workspace(lib, num_parts, seq_lens.shape[0], int(max_new_len), num_kv_heads,
+                                                         int(max_context_len), query)
+        _check(lib.sw_context_attention_scaled(
+            out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
+            value_scales.data_ptr(), seq_lens.shape[0], rows, num_heads, num_kv_heads, head_size, float(scale),
+            block_tables.data_ptr(), seq_starts.data_ptr(), new_lens.data_ptr(), seq_lens.data_ptr(), value_cache.shape[3],
+            value_cache.shape[0], int(max_new_len), int(max_context_len), block_tables.shape[1], block_tables.stride(0),
+            alibi_slopes.data_ptr() if alibi_slopes is not None else None, int(sliding_window) if sliding_window else 0,
+            query.stride(0), out.stride(0), _act_dtype(query), cache, num_parts, workspace.data_ptr() if nbytes else None, nbytes,
+            _stream(query)))
+
+
 def _rows(t: torch.Tensor):
     """(number of rows, row stride in elements) of a tensor whose last dim is contiguous and whose
     leading dims collapse to one stride."""
@@ -933,6 +1124,8 @@ ops = SimpleNamespace(
     prefill_attention=prefill_attention,
     prefill_attention_and_cache=prefill_attention_and_cache,
     context_attention_fwd=context_attention_fwd,
+    paged_attention_scaled=paged_attention_scaled,
+    context_attention_scaled=context_attention_scaled,
     rms_norm=rms_norm,
     fused_add_rms_norm=fused_add_rms_norm,
     rotary_embedding=rotary_embedding,
@@ -952,6 +1145,8 @@ cache_ops = SimpleNamespace(
     copy_blocks=copy_blocks,
     swap_blocks=swap_blocks,
     convert_fp8_e5m2=convert_fp8_e5m2,
+    reshape_and_cache_scaled=reshape_and_cache_scaled,
+    gather_cache_scaled=gather_cache_scaled,
 )
 custom_ar = SimpleNamespace(
     signal_bytes=custom_ar_signal_bytes,
