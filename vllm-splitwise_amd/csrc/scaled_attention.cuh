@@ -18,7 +18,7 @@ struct ScAttention {
   int64_t q_stride, out_stride, num_rows, table_stride;
   int num_blocks, width, heads, kv_heads, group, head_size;
   int window;                      // 0: none
-  int part_tokens, parts, tiles, most_new;
+  int part_tokens, parts, tiles, tile_rows, most_new;
   float scale2;                    // the softmax's scale times log2(e): everything below is in powers of two
   bool bf16;
 };

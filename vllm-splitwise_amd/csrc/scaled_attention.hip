@@ -8,6 +8,8 @@ namespace sw {
 
 int sc_decode_i8(const ScAttention& a, int block_size, int num_seqs, hipStream_t stream);
 int sc_decode_e4m3(const ScAttention& a, int block_size, int num_seqs, hipStream_t stream);
+int sc_context_i8(const ScAttention& a, int block_size, int num_seqs, hipStream_t stream);
+int sc_context_e4m3(const ScAttention& a, int block_size, int num_seqs, hipStream_t stream);
 
 namespace {
 
@@ -17,8 +19,9 @@ __global__ void __launch_bounds__(256) scaled_join_kernel(const ScAttention a) {
   const int seq = blockIdx.z, tok = blockIdx.x, head = blockIdx.y, d = threadIdx.x;
   const ScSequence s = sc_sequence<BS>(a, seq);
   if (tok >= s.fresh) return;
-  const int rows = s.fresh * a.group, mine = tok * a.group + head % a.group, tile = mine / 16;
-  const int pos_low = s.first + tile * 16 / a.group, pos_high = s.first + min(rows - 1, tile * 16 + 15) / a.group;
+  const int rows = s.fresh * a.group, mine = tok * a.group + head % a.group, tile = mine / a.tile_rows;
+  const int pos_low = s.first + tile * a.tile_rows / a.group;
+  const int pos_high = s.first + min(rows - 1, tile * a.tile_rows + a.tile_rows - 1) / a.group;
   const int from = sc_seen_from(a, pos_low);
   const int64_t row = s.row0 + tok;
   const float* parts = a.partial + (row * a.heads + head) * a.parts * (a.head_size + 4);
@@ -41,6 +44,9 @@ __global__ void __launch_bounds__(256) scaled_join_kernel(const ScAttention a) {
       a.bf16 ? float_to_bf16_bits(res) : float_to_f16_bits(res);
 }
 
+// Rows of a tile for `rows` rows of a (sequence, kv head): 16 of the kernel for few rows or 128 of the one for many.
+int sc_tile_rows(int64_t rows) { return rows <= 16 ? 16 : 128; }
+
 int sc_attend(const char* what, ScAttention a, int num_seqs, int64_t num_blocks, int block_size, int max_new_len, int max_context_len,
               int act, int cache, int num_parts, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
   SW_CHECK_ARG(cache == SW_I8_SCALED || cache == SW_E4M3_SCALED, "%s: the cache type must be scaled int8 or e4m3", what);
@@ -62,7 +68,8 @@ int sc_attend(const char* what, ScAttention a, int num_seqs, int64_t num_blocks,
                                   workspace_bytes >= sw_scaled_attention_workspace_bytes(num_parts, a.num_rows, a.heads, a.head_size)),
                "%s: the workspace for %d parts is missing, too small or not aligned", what, num_parts);
   a.group = a.heads / a.kv_heads;
-  const int64_t tiles = ((int64_t)max_new_len * a.group + 15) / 16;
+  a.tile_rows = sc_tile_rows((int64_t)max_new_len * a.group);
+  const int64_t tiles = ((int64_t)max_new_len * a.group + a.tile_rows - 1) / a.tile_rows;
   SW_CHECK_ARG((int64_t)max_new_len * a.group < INT32_MAX / 2 && tiles * a.kv_heads <= INT32_MAX, "%s: %d new tokens", what, max_new_len);
   if (num_seqs == 0 || max_new_len == 0 || a.num_rows == 0) return SW_OK;
   a.num_blocks = (int)num_blocks;
@@ -71,7 +78,9 @@ int sc_attend(const char* what, ScAttention a, int num_seqs, int64_t num_blocks,
   a.part_tokens = num_parts == 1 ? 0 : std::max(64, (int)((((int64_t)max_context_len + num_parts - 1) / num_parts + 63) / 64 * 64));
   a.partial = num_parts == 1 ? nullptr : (float*)workspace;
   a.bf16 = act == SW_BF16;
-  const int rc = cache == SW_E4M3_SCALED ? sc_decode_e4m3(a, block_size, num_seqs, stream) : sc_decode_i8(a, block_size, num_seqs, stream);
+  const bool e4m3 = cache == SW_E4M3_SCALED;
+  const int rc = a.tile_rows == 16 ? (e4m3 ? sc_decode_e4m3 : sc_decode_i8)(a, block_size, num_seqs, stream)
+                                   : (e4m3 ? sc_context_e4m3 : sc_context_i8)(a, block_size, num_seqs, stream);
   if (rc != SW_OK || num_parts == 1) return rc;
   const dim3 grid(max_new_len, a.heads, num_seqs);
   const int threads = (a.head_size + 63) / 64 * 64;
@@ -105,7 +114,8 @@ extern "C" {
 
 int sw_scaled_attention_parts(int num_seqs, int max_new_len, int num_heads, int num_kv_heads, int head_size, int max_context_len) {
   if (num_seqs <= 0 || max_new_len <= 0 || num_kv_heads <= 0 || num_heads < num_kv_heads || max_context_len <= 0) return 1;
-  const int64_t tiles = ((int64_t)max_new_len * (num_heads / num_kv_heads) + 15) / 16;
+  const int64_t rows = (int64_t)max_new_len * (num_heads / num_kv_heads), tile = sw::sc_tile_rows(rows);
+  const int64_t tiles = (rows + tile - 1) / tile;
   const int64_t workgroups = (int64_t)num_seqs * num_kv_heads * tiles;
   const int64_t most = ((int64_t)max_context_len + 255) / 256;
   return (int)std::max<int64_t>(1, std::min<int64_t>(most, 1024 / workgroups));
