@@ -23,6 +23,8 @@ constexpr int kScWaves = 4, kScRows = 32, kScTileRows = kScWaves * kScRows;
 constexpr float kScLazy = 8.f;                                // powers of two by which a weight may pass 1
 constexpr float kScDeep = 40.f;                               // below the reference by more a value scale counts as that much below it
 
+constexpr int kScSteps = 8;                                   // dwords of codes of a key's piece and a value's
+
 __host__ __device__ constexpr int sc_stage(int head) { return head <= 128 ? 64 : 32; }
 __host__ __device__ constexpr int sc_padded(int head) { return (head + 31) / 32 * 32; }
 __host__ __device__ constexpr int sc_kstride(int head) { return head * 2 + 16; }            // bytes; 16 rows on 64 banks
@@ -35,7 +37,6 @@ template <bool E4M3, int HEAD, int BS>
 __global__ void __launch_bounds__(kScWaves * 64, 2) scaled_context_kernel(const ScAttention a) {
   using C = ScCode<E4M3>;
   constexpr int KT = sc_stage(HEAD), NT = KT / 32, KS = HEAD / 16, DB = sc_padded(HEAD) / 32;
-  constexpr int THREADS = kScWaves * 64, PIECES = KT * HEAD / 16, NP = (PIECES + THREADS - 1) / THREADS;
   constexpr int KSTRIDE = sc_kstride(HEAD), VSTRIDE = sc_vstride(HEAD), BUFFER = sc_buffer(HEAD);
   constexpr int PB = BS == 8 ? 2 : 1, SB = KT / 8;            // blocks of a run of 16 tokens; eights of a stage
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -103,84 +104,86 @@ __global__ void __launch_bounds__(kScWaves * 64, 2) scaled_context_kernel(const 
   }
   const float slope = a.slopes ? a.slopes[head] * 1.44269504088896340736f : 0.f;
 
-  // ---- staging
+  // ---- staging: a wave brings one run of 16 tokens (half of one, where there are fewer runs than waves), so that its blocks are the same
+  // for all its lanes; a lane's pieces are 16 dims of one token's key and 16 tokens of one dim's values
   const int64_t head_bytes = (int64_t)HEAD * BS, block_bytes = head_bytes * a.kv_heads;
   const uint8_t* const k_base = a.key_cache + kv_head * head_bytes;
   const uint8_t* const v_base = a.value_cache + kv_head * head_bytes;
   const int32_t* table = a.tables + (int64_t)seq * a.table_stride;
   const int last_block = (s.len - 1) / BS;
+  constexpr int RUNS = KT / 16, SHARE = kScWaves / RUNS, NP = (HEAD + 64 * SHARE - 1) / (64 * SHARE);
+  const int run = wave / SHARE, u0 = (wave % SHARE) * 64 + lane;
+  auto mine = [&](int i) { return HEAD % (64 * SHARE) == 0 || u0 + i * 64 * SHARE < HEAD; };
+  // (stages behind the last one bring the last block again: what they lay down is not read)
   auto entry = [&](int t) -> int { return table[min(t / BS, last_block)]; };
-  auto exists = [&](int b) { return b >= 0 && b < a.num_blocks; };
-  // a thread's pieces: 16 dims of token kt[i] of the stage; dim vd[i] of the tokens of run vr[i]
-  int kblock[NP], vblock[NP][PB], sblock = 0;                 // their blocks, one stage further ahead than the pieces
-  sc_u32x4 kraw[NP], vraw[NP];
+  int runblock[PB], sblock = 0;                               // one stage further ahead than the pieces
+  sc_u32x4 kraw[NP], vraw[NP], keep = {0u, 0u, 0u, 0u};
   float kscale = 0.f, vscale = 0.f;
   bool sgood = false;
   float reference = -INFINITY;                                // of threads 0 .. SB - 1: log2 of the largest value scale so far
-  auto k_token = [&](int u) { return (u / 16 / KS) * 16 + u % 16; };
   auto look = [&](int t0) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int u = i * THREADS + tid;
-      if (PIECES % THREADS != 0 && u >= PIECES) continue;
-      kblock[i] = entry(t0 + k_token(u));
-#pragma unroll
-      for (int b = 0; b < PB; ++b) vblock[i][b] = entry(t0 + (u / HEAD) * 16 + 8 * b);
-    }
+    for (int b = 0; b < PB; ++b) runblock[b] = entry(t0 + 16 * run + 8 * b);
     if (tid < SB) sblock = entry(t0 + 8 * tid);
   };
   auto fetch = [&](int t0) {
+    const int off = (t0 + 16 * run) % BS;                     // of the run in its block
+    bool good[PB];
+    int64_t at[PB];
+#pragma unroll
+    for (int b = 0; b < PB; ++b) {
+      good[b] = runblock[b] >= 0 && runblock[b] < a.num_blocks;
+      at[b] = (good[b] ? runblock[b] : 0) * block_bytes;
+    }
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int u = i * THREADS + tid;
-      if (PIECES % THREADS != 0 && u >= PIECES) continue;
-      {
-        const int off = (t0 + k_token(u)) % BS, c = u / 16 % KS;
-        const int b = exists(kblock[i]) ? kblock[i] : 0;
-        kraw[i] = *reinterpret_cast<const sc_u32x4*>(k_base + b * block_bytes + (c * BS + off) * 16);
-      }
-      const int d = u % HEAD, off = (t0 + (u / HEAD) * 16) % BS;
+      if (!mine(i)) continue;
+      const int u = u0 + i * 64 * SHARE, t = u & 15, c = u >> 4;
       if constexpr (PB == 2) {
-        sc_u32x2 w[2];
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-          w[b] = exists(vblock[i][b]) ? *reinterpret_cast<const sc_u32x2*>(v_base + vblock[i][b] * block_bytes + d * BS) : sc_u32x2{0u, 0u};
-        vraw[i] = sc_join(w[0], w[1]);
+        kraw[i] = *reinterpret_cast<const sc_u32x4*>(k_base + (t < 8 ? at[0] : at[1]) + (c * BS + (t & 7)) * 16);
+        vraw[i] = sc_join(*reinterpret_cast<const sc_u32x2*>(v_base + at[0] + u * BS), *reinterpret_cast<const sc_u32x2*>(v_base + at[1] + u * BS));
       } else {
-        vraw[i] = exists(vblock[i][0]) ? *reinterpret_cast<const sc_u32x4*>(v_base + vblock[i][0] * block_bytes + d * BS + off)
-                                       : sc_u32x4{0u, 0u, 0u, 0u};
+        kraw[i] = *reinterpret_cast<const sc_u32x4*>(k_base + at[0] + off * 16 + (c * BS + t) * 16);
+        vraw[i] = *reinterpret_cast<const sc_u32x4*>(v_base + at[0] + off + u * BS);
       }
     }
     if (tid < SB) {
-      sgood = exists(sblock);
+      sgood = sblock >= 0 && sblock < a.num_blocks;
       kscale = sgood ? a.key_scales[(int64_t)sblock * a.kv_heads + kv_head] : 0.f;
       vscale = sgood ? a.value_scales[(int64_t)sblock * a.kv_heads + kv_head] : 0.f;
     }
+    // slots that hold no token may hold a NaN's code: which of the run's values are kept
+    if constexpr (E4M3) {
+      const int left = s.len - t0 - 16 * run;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int n = left - 4 * w;
+        keep[w] = !good[PB == 2 ? w >> 1 : 0] || n <= 0 ? 0u : n >= 4 ? 0xffffffffu : (1u << (8 * n)) - 1u;
+      }
+    }
   };
-  auto commit = [&](int t0, int buf) {
+  // widening and laying down, one of kScSteps * NP steps: a dword of codes each, 16 bytes stored with every second one
+  sc_u32x2 held;
+  auto lay_step = [&](auto K, int buf) {
+    constexpr int i = decltype(K)::value / kScSteps, j = decltype(K)::value % kScSteps, w = j < 4 ? j : j == 5 ? 2 : j == 6 ? 1 : j & 3;
+    if (!mine(i)) return;
     char* k_img = smem + buf * BUFFER;
     char* v_img = k_img + KT * KSTRIDE;
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int u = i * THREADS + tid;
-      if (PIECES % THREADS != 0 && u >= PIECES) continue;
-      sc_u32x4* kp = reinterpret_cast<sc_u32x4*>(k_img + k_token(u) * KSTRIDE + (u / 16 % KS) * 32);
-      kp[0] = sc_join(C::widen(kraw[i][0]), C::widen(kraw[i][1]));
-      kp[1] = sc_join(C::widen(kraw[i][2]), C::widen(kraw[i][3]));
-      const int run = u / HEAD;
-      sc_u32x4 v = vraw[i];
-      if (E4M3 && t0 + KT > s.len) {                          // slots that hold no token may hold a NaN's code
-        const int left = s.len - t0 - 16 * run;
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          v[w] = left >= 4 * w + 4 ? v[w] : left <= 4 * w ? 0u : v[w] & ((1u << (8 * (left - 4 * w))) - 1u);
-      }
-      sc_u32x4* vp = reinterpret_cast<sc_u32x4*>(v_img + (u % HEAD) * VSTRIDE + run * 32);
-      vp[0] = sc_join(C::widen(v[0]), C::widen(v[2]));
-      vp[1] = sc_join(C::widen(v[1]), C::widen(v[3]));
+    const int u = u0 + i * 64 * SHARE;
+    uint32_t code = j < 4 ? kraw[i][w] : vraw[i][w];
+    if constexpr (E4M3 && j >= 4) code &= keep[w];
+    const sc_u32x2 wide = C::widen(code);
+    if constexpr (j % 2 == 0) {
+      held = wide;
+    } else {
+      char* to = j < 4 ? k_img + (16 * run + (u & 15)) * KSTRIDE + (u >> 4) * 32 : v_img + u * VSTRIDE + run * 32;
+      *reinterpret_cast<sc_u32x4*>(to + (j & 2) * 8) = sc_join(held, wide);
     }
+  };
+  auto lay = [&](int buf) { static_for<kScSteps * NP>([&](auto K) { lay_step(K, buf); }); };
+  auto lay_scales = [&](int t0, int buf) {
     if (tid < SB) {
-      float* f = reinterpret_cast<float*>(v_img + sc_padded(HEAD) * VSTRIDE);
+      float* f = reinterpret_cast<float*>(smem + buf * BUFFER + KT * KSTRIDE + sc_padded(HEAD) * VSTRIDE);
       const float there = t0 + 8 * tid < s.len && vscale > 0.f ? __builtin_amdgcn_logf(vscale) : -INFINITY;
       float top = there;
 #pragma unroll
@@ -210,23 +213,22 @@ __global__ void __launch_bounds__(kScWaves * 64, 2) scaled_context_kernel(const 
   if (stages > 0) {
     look(first);
     fetch(first);
-    if (stages > 1) look(first + KT);
-    commit(first, 0);
-    if (stages > 1) {
-      fetch(first + KT);
-      if (stages > 2) look(first + 2 * KT);
-    }
+    look(first + KT);
+    lay(0);
+    lay_scales(first, 0);
+    fetch(first + KT);
+    look(first + 2 * KT);
     __syncthreads();
   }
   int buf = 0;
   for (int st = 0; st < stages; ++st, buf ^= 1) {
     const int t0 = first + st * KT;
-    if (st + 1 < stages) commit(t0 + KT, buf ^ 1);
-    if (st + 2 < stages) {
+    lay_scales(t0 + KT, buf ^ 1);
+    if (!(active && t0 <= wave_high && t0 + KT > wave_from)) {
+      lay(buf ^ 1);
       fetch(t0 + 2 * KT);
-      if (st + 3 < stages) look(t0 + 3 * KT);
-    }
-    if (active && t0 <= wave_high && t0 + KT > wave_from) {
+      look(t0 + 3 * KT);
+    } else {
       const char* k_img = smem + buf * BUFFER;
       const char* v_img = k_img + KT * KSTRIDE;
       const float* f = reinterpret_cast<const float*>(v_img + sc_padded(HEAD) * VSTRIDE);
@@ -236,12 +238,24 @@ __global__ void __launch_bounds__(kScWaves * 64, 2) scaled_context_kernel(const 
       for (int u = 0; u < NT; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[u][i] = 0.f;
+      // The scores' products, their operands read three ahead, and between them the next stage's widening: the order is held.
+      {
+        auto operand = [&](int n) { return *reinterpret_cast<const sc_f16x8*>(kp + n % NT * 32 * KSTRIDE + n / NT * 32); };
+        constexpr int N = NT * KS, AHEAD = 3, STEPS = kScSteps * NP;
+        sc_f16x8 ring[AHEAD + 1];
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int u = 0; u < NT; ++u)
-          x[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const sc_f16x8*>(kp + u * 32 * KSTRIDE + ks * 32),
-                                                        __builtin_bit_cast(sc_f16x8, qf[ks]), x[u], 0, 0, 0);
+        for (int n = 0; n < AHEAD; ++n) ring[n] = operand(n);
+        static_for<N>([&](auto I) {
+          constexpr int n = decltype(I)::value;
+          if constexpr (n + AHEAD < N) ring[(n + AHEAD) % (AHEAD + 1)] = operand(n + AHEAD);
+          x[n % NT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[n % (AHEAD + 1)], __builtin_bit_cast(sc_f16x8, qf[n / NT]), x[n % NT], 0, 0, 0);
+          static_for<STEPS*(n + 1) / N - STEPS * n / N>(
+              [&](auto K) { lay_step(std::integral_constant<int, STEPS * n / N + decltype(K)::value>{}, buf ^ 1); });
+          __builtin_amdgcn_sched_barrier(0);
+        });
+      }
+      fetch(t0 + 2 * KT);
+      look(t0 + 3 * KT);
 
       // scores in powers of two: x fs (+ nothing more, where no row has anything to hide or to add)
       float fs[SB];
@@ -283,27 +297,42 @@ __global__ void __launch_bounds__(kScWaves * 64, 2) scaled_context_kernel(const 
           for (int i = 0; i < 16; ++i) o[b][i] *= shrink;
       }
       const float base = sc_base(m_run);
-      sc_u32x4 pf[NT][2];
-#pragma unroll
-      for (int b = 0; b < SB; ++b) {
-        const int u = b >> 2, i = (b & 3) * 4;
-        const float c = f[8 + b] - base;
-        float p[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(x[u][i + j], fs[b], c));
-        l_run = fmaf((p[0] + p[1]) + (p[2] + p[3]), f[16 + b], l_run);
-        pf[u][(b & 3) >> 1][2 * (b & 1)] = sc_pack_f16(p[0], p[1]);
-        pf[u][(b & 3) >> 1][2 * (b & 1) + 1] = sc_pack_f16(p[2], p[3]);
-      }
+      // Weights of a run of 16 tokens, a few between each two products of the run before.
       const char* vp = v_img + col * VSTRIDE + half * 16;
+      constexpr int RN = 2 * NT;
+      float p[8], shift = 0.f;
+      sc_u32x4 pf;
+      auto weigh = [&](auto N_, auto E) {
+        constexpr int n = decltype(N_)::value, e = decltype(E)::value, b = 2 * n + e / 4;
+        if constexpr (e % 4 == 0) shift = f[8 + b] - base;
+        p[e] = __builtin_amdgcn_exp2f(fmaf(x[b >> 2][(b & 3) * 4 + e % 4], fs[b], shift));
+      };
+      auto pack = [&](auto N_) {
+        constexpr int n = decltype(N_)::value;
+        l_run = fmaf((p[0] + p[1]) + (p[2] + p[3]), f[16 + 2 * n], l_run);
+        l_run = fmaf((p[4] + p[5]) + (p[6] + p[7]), f[17 + 2 * n], l_run);
 #pragma unroll
-      for (int u = 0; u < NT; ++u)
+        for (int w = 0; w < 4; ++w) pf[w] = sc_pack_f16(p[2 * w], p[2 * w + 1]);
+      };
+      auto operand = [&](int n) { return *reinterpret_cast<const sc_f16x8*>(vp + n % DB * 32 * VSTRIDE + n / DB * 32); };
+      constexpr int AHEAD = 2;
+      sc_f16x8 ring[AHEAD + 1];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int b = 0; b < DB; ++b)
-            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const sc_f16x8*>(vp + b * 32 * VSTRIDE + u * 64 + h * 32),
-                                                          __builtin_bit_cast(sc_f16x8, pf[u][h]), o[b], 0, 0, 0);
+      for (int n = 0; n < AHEAD; ++n) ring[n] = operand(n);
+      static_for<8>([&](auto E) { weigh(std::integral_constant<int, 0>{}, E); });
+      pack(std::integral_constant<int, 0>{});
+      static_for<RN * DB>([&](auto I) {
+        constexpr int i = decltype(I)::value, n = i / DB, b = i % DB;
+        if constexpr (i + AHEAD < RN * DB) ring[(i + AHEAD) % (AHEAD + 1)] = operand(i + AHEAD);
+        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[i % (AHEAD + 1)], __builtin_bit_cast(sc_f16x8, pf), o[b], 0, 0, 0);
+        if constexpr (n + 1 < RN) {
+          static_for<8 * (b + 1) / DB - 8 * b / DB>([&](auto E) {
+            weigh(std::integral_constant<int, n + 1>{}, std::integral_constant<int, 8 * b / DB + decltype(E)::value>{});
+          });
+          if constexpr (b == DB - 1) pack(std::integral_constant<int, n + 1>{});
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      });
     }
     __syncthreads();
   }
