@@ -6,46 +6,138 @@
 
 namespace sw {
 
-int sc_decode_i8(const ScAttention& a, int block_size, int num_seqs, hipStream_t stream);
-int sc_decode_e4m3(const ScAttention& a, int block_size, int num_seqs, hipStream_t stream);
-int sc_context_i8(const ScAttention& a, int block_size, int num_seqs, hipStream_t stream);
-int sc_context_e4m3(const ScAttention& a, int block_size, int num_seqs, hipStream_t stream);
+using ScLaunch = int(const ScAttention& a, int block_size, int num_seqs, hipStream_t stream);
+ScLaunch sc_decode_i8, sc_decode_i8_wide, sc_decode_e4m3, sc_decode_e4m3_wide, sc_context_i8, sc_context_i8_wide, sc_context_e4m3,
+    sc_context_e4m3_wide;
 
 namespace {
 
-// One workgroup for each (row, head): o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p over the parts that its tile had.
+constexpr int kScMostParts = 1024;
+
+// One workgroup for each (row, head): o = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p over the parts that its tile had.  A wave
+// finds the factors, a part a lane; then 8 groups of 32 threads take every 8th part, 4 dims a thread (twice for heads over 128), and
+// are added up through LDS.
+constexpr int kScJoinThreads = 256;
+
 template <int BS>
-__global__ void __launch_bounds__(256) scaled_join_kernel(const ScAttention a) {
-  const int seq = blockIdx.z, tok = blockIdx.x, head = blockIdx.y, d = threadIdx.x;
+__global__ void __launch_bounds__(kScJoinThreads) scaled_join_kernel(const ScAttention a) {
+  __shared__ float factor[kScMostParts];
+  __shared__ sc_f32x4 sums[kScJoinThreads];
+  const int seq = blockIdx.z, tok = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
   const ScSequence s = sc_sequence<BS>(a, seq);
   if (tok >= s.fresh) return;
   const int rows = s.fresh * a.group, mine = tok * a.group + head % a.group, tile = mine / a.tile_rows;
   const int pos_low = s.first + tile * a.tile_rows / a.group;
   const int pos_high = s.first + min(rows - 1, tile * a.tile_rows + a.tile_rows - 1) / a.group;
   const int from = sc_seen_from(a, pos_low);
-  const int64_t row = s.row0 + tok;
-  const float* parts = a.partial + (row * a.heads + head) * a.parts * (a.head_size + 4);
-  const int64_t step = a.head_size + 4;
+  const int64_t row = s.row0 + tok, step = a.head_size + 4;
+  const float* parts = a.partial + (row * a.heads + head) * a.parts * step;
   auto there = [&](int p) { return max(p * a.part_tokens, from) < sc_part_end(a, s, p, pos_high); };
-  float m = -INFINITY;
-  for (int p = 0; p < a.parts; ++p)
-    if (there(p)) m = fmaxf(m, parts[p * step + a.head_size]);
-  const float base = sc_base(m);
-  float l = 0.f, o = 0.f;
-  for (int p = 0; p < a.parts; ++p) {
-    if (!there(p)) continue;
-    const float f = __builtin_amdgcn_exp2f(parts[p * step + a.head_size] - base);
-    l += parts[p * step + a.head_size + 1] * f;
-    if (d < a.head_size) o += parts[p * step + d] * f;
+  if (tid < 64) {
+    float m = -INFINITY, l = 0.f;
+    for (int p = tid; p < a.parts; p += 64)
+      if (there(p)) m = fmaxf(m, parts[p * step + a.head_size]);
+    const float base = sc_base(wave_max(m));
+    for (int p = tid; p < a.parts; p += 64) {
+      const float f = there(p) ? __builtin_amdgcn_exp2f(parts[p * step + a.head_size] - base) : 0.f;
+      if (there(p)) l += parts[p * step + a.head_size + 1] * f;
+      factor[p] = f;
+    }
+    l = wave_sum(l);
+    const float inv = l > 0.f ? 1.f / l : l != l ? l : 0.f;     // a row that sees nothing gives zeros
+    for (int p = tid; p < a.parts; p += 64) factor[p] *= inv;
   }
-  if (d >= a.head_size) return;
-  const float res = l > 0.f ? o / l : l != l ? l : 0.f;
-  reinterpret_cast<uint16_t*>(a.out)[row * a.out_stride + (int64_t)head * a.head_size + d] =
-      a.bf16 ? float_to_bf16_bits(res) : float_to_f16_bits(res);
+  __syncthreads();
+  for (int d = 4 * (tid & 31); d < (a.head_size + 127) / 128 * 128; d += 128) {
+    sc_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    if (d < a.head_size) {
+#pragma unroll 4
+      for (int p = tid >> 5; p < a.parts; p += 8)
+        if (there(p)) o += *reinterpret_cast<const sc_f32x4*>(parts + p * step + d) * factor[p];
+    }
+    sums[tid] = o;
+    __syncthreads();
+    if (tid < 32 && d < a.head_size) {
+#pragma unroll
+      for (int g = 1; g < kScJoinThreads / 32; ++g) o += sums[tid + 32 * g];
+      *reinterpret_cast<sc_u32x2*>(reinterpret_cast<uint16_t*>(a.out) + row * a.out_stride + (int64_t)head * a.head_size + d) =
+          sc_u32x2{sc_pack16(o[0], o[1], a.bf16), sc_pack16(o[2], o[3], a.bf16)};
+    }
+    __syncthreads();
+  }
 }
 
-// Rows of a tile for `rows` rows of a (sequence, kv head): 16 of the kernel for few rows or 128 of the one for many.
-int sc_tile_rows(int64_t rows) { return rows <= 16 ? 16 : 128; }
+// The same for few parts of many rows: a wave for each (row, head), 4 dims a lane.
+template <int BS>
+__global__ void __launch_bounds__(256) scaled_join_few_kernel(const ScAttention a) {
+  const int seq = blockIdx.z, tok = blockIdx.x, lane = threadIdx.x & 63;
+  const int head = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const ScSequence s = sc_sequence<BS>(a, seq);
+  if (tok >= s.fresh || head >= a.heads) return;
+  const int rows = s.fresh * a.group, mine = tok * a.group + head % a.group, tile = mine / a.tile_rows;
+  const int pos_low = s.first + tile * a.tile_rows / a.group;
+  const int pos_high = s.first + min(rows - 1, tile * a.tile_rows + a.tile_rows - 1) / a.group;
+  const int from = sc_seen_from(a, pos_low);
+  const int64_t row = s.row0 + tok, step = a.head_size + 4;
+  const float* parts = a.partial + (row * a.heads + head) * a.parts * step;
+  auto there = [&](int p) { return max(p * a.part_tokens, from) < sc_part_end(a, s, p, pos_high); };
+  float m = -INFINITY, l = 0.f;
+  sc_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  const bool mine_d = 4 * lane < a.head_size;
+  for (int p = 0; p < a.parts; ++p) {
+    if (!there(p)) continue;
+    const float* at = parts + p * step;
+    const sc_f32x4 v = mine_d ? *reinterpret_cast<const sc_f32x4*>(at + 4 * lane) : sc_f32x4{0.f, 0.f, 0.f, 0.f};
+    const float mp = at[a.head_size], lp = at[a.head_size + 1], m_new = fmaxf(m, mp), base = sc_base(m_new);
+    const float f = __builtin_amdgcn_exp2f(m - base), g = __builtin_amdgcn_exp2f(mp - base);
+    m = m_new;
+    l = l * f + lp * g;
+    o = o * f + v * g;
+  }
+  const float inv = l > 0.f ? 1.f / l : l != l ? l : 0.f;     // a row that sees nothing gives zeros
+  if (mine_d)
+    *reinterpret_cast<sc_u32x2*>(reinterpret_cast<uint16_t*>(a.out) + row * a.out_stride + (int64_t)head * a.head_size + 4 * lane) =
+        sc_u32x2{sc_pack16(o[0] * inv, o[1] * inv, a.bf16), sc_pack16(o[2] * inv, o[3] * inv, a.bf16)};
+}
+
+template <int BS>
+void sc_join(const ScAttention& a, int max_new_len, int num_seqs, hipStream_t stream) {
+  if (a.parts <= 8) scaled_join_few_kernel<BS><<<dim3(max_new_len, (a.heads + 3) / 4, num_seqs), 256, 0, stream>>>(a);
+  else scaled_join_kernel<BS><<<dim3(max_new_len, a.heads, num_seqs), kScJoinThreads, 0, stream>>>(a);
+}
+
+// What a call of some shape launches: which kernel, on tiles of how many rows (16: the one for few rows, else the one for many), with
+// how many waves a workgroup, and over how many parts of a context.
+struct ScPlan { int tile_rows, waves, parts; };
+
+ScPlan sc_plan(int num_seqs, int max_new_len, int num_heads, int num_kv_heads, int head_size, int max_context_len) {
+  ScPlan p;
+  const int64_t rows = (int64_t)max_new_len * (num_heads / num_kv_heads), pairs = (int64_t)num_seqs * num_kv_heads;
+  auto workgroups = [&](int tile) { return std::max<int64_t>(1, pairs * ((rows + tile - 1) / tile)); };
+  // Rows of 16: all tiles of a kv head read its codes again, from the L2 but for the first, and are many workgroups where the others are
+  // few (us, 16 / 128 rows: 15 x 8 tokens of 8 heads behind 1803 38 / 56, 1 x 40 behind 4000 36 / 35, 16 x 21 behind 2000 54 / 77,
+  // 2 x 159 of one head behind 4000 84 / 67, 8 x 214 behind 1000 83 / 65).
+  if (rows <= (head_size > 128 ? 16 : 96) || (head_size <= 128 && rows <= 160 && workgroups(16) >= 1024)) {
+    p.tile_rows = 16;
+    // Few workgroups take 8 waves; a context is shared out until there are about 256 of them (us, 8 waves by parts: 1 x 2001 tokens of 8
+    // kv heads 1 17.2, 4 12.2, 8 10.9, 32 11.9; 4 x 6001 1 60.9, 4 25.5, 8 18.1, 16 23.1; 32 heads, 1 x 501 1 8.6, 2 10.6; 4 and 8 waves:
+    // 64 x 1000 of 8 heads 38.9 / 41.5, 32 x 8192 143 / 117, 128 x 4096 220 / 212).
+    const int64_t w = workgroups(16);
+    p.waves = head_size <= 128 && w <= (max_context_len >= 4096 ? 1024 : 256) ? 8 : 4;
+    p.parts = (int)std::min<int64_t>(max_context_len < 1024 ? 1 : ((int64_t)max_context_len + 255) / 256, 256 / w);
+  } else {
+    // 256 rows where there are enough of them: half the widening a row (us, 128 / 256 rows: 2041 tokens of 8 heads behind 14003 1127 /
+    // 1040, 8 x 1024 behind 1000 372 / 372, 6 x 301 89 / 87, 30 x 50 behind 10 35 / 39; heads of 64 153 / 169, of 256 554 / 563).
+    // Fewer: parts, for whose sums each row costs 2 x 4 bytes a dim and part (500 tokens of 32 heads behind 4000, 1 / 2 / 4 / 8 parts: 138 / 88 /
+    // 70 / 83; 1000 of 32 heads behind 100, 1 / 2: 46 / 53).
+    const int64_t w = workgroups(128);
+    p.tile_rows = head_size >= 80 && head_size <= 128 && w >= 512 && max_context_len >= 1024 ? 256 : 128;
+    p.waves = p.tile_rows / 32;
+    p.parts = w >= 512 ? 1 : (int)std::min<int64_t>(max_context_len / 768, (512 + w / 2) / w);
+  }
+  p.parts = std::max(1, std::min(p.parts, kScMostParts));
+  return p;
+}
 
 int sc_attend(const char* what, ScAttention a, int num_seqs, int64_t num_blocks, int block_size, int max_new_len, int max_context_len,
               int act, int cache, int num_parts, void* workspace, int64_t workspace_bytes, hipStream_t stream) {
@@ -63,14 +155,16 @@ int sc_attend(const char* what, ScAttention a, int num_seqs, int64_t num_blocks,
   SW_CHECK_ARG((uintptr_t)a.query % 16 == 0 && a.q_stride % 8 == 0 && (uintptr_t)a.out % 16 == 0 && a.out_stride % 8 == 0 &&
                    (uintptr_t)a.key_cache % 16 == 0 && (uintptr_t)a.value_cache % 16 == 0,
                "%s: rows of query and out, and the caches, must begin on multiples of 16 bytes", what);
-  SW_CHECK_ARG(num_parts >= 1 && num_parts <= 65535, "%s: %d parts", what, num_parts);
+  SW_CHECK_ARG(num_parts >= 1 && num_parts <= kScMostParts, "%s: %d parts, at most %d", what, num_parts, kScMostParts);
   SW_CHECK_ARG(num_parts == 1 || (workspace && (uintptr_t)workspace % 16 == 0 &&
                                   workspace_bytes >= sw_scaled_attention_workspace_bytes(num_parts, a.num_rows, a.heads, a.head_size)),
                "%s: the workspace for %d parts is missing, too small or not aligned", what, num_parts);
   a.group = a.heads / a.kv_heads;
-  a.tile_rows = sc_tile_rows((int64_t)max_new_len * a.group);
+  SW_CHECK_ARG((int64_t)max_new_len * a.group < INT32_MAX / 2, "%s: %d new tokens", what, max_new_len);
+  const ScPlan plan = sc_plan(num_seqs, max_new_len, a.heads, a.kv_heads, a.head_size, max_context_len);
+  a.tile_rows = plan.tile_rows;
   const int64_t tiles = ((int64_t)max_new_len * a.group + a.tile_rows - 1) / a.tile_rows;
-  SW_CHECK_ARG((int64_t)max_new_len * a.group < INT32_MAX / 2 && tiles * a.kv_heads <= INT32_MAX, "%s: %d new tokens", what, max_new_len);
+  SW_CHECK_ARG(tiles * a.kv_heads <= INT32_MAX, "%s: %d new tokens", what, max_new_len);
   if (num_seqs == 0 || max_new_len == 0 || a.num_rows == 0) return SW_OK;
   a.num_blocks = (int)num_blocks;
   a.tiles = (int)tiles;
@@ -79,14 +173,13 @@ int sc_attend(const char* what, ScAttention a, int num_seqs, int64_t num_blocks,
   a.partial = num_parts == 1 ? nullptr : (float*)workspace;
   a.bf16 = act == SW_BF16;
   const bool e4m3 = cache == SW_E4M3_SCALED;
-  const int rc = a.tile_rows == 16 ? (e4m3 ? sc_decode_e4m3 : sc_decode_i8)(a, block_size, num_seqs, stream)
-                                   : (e4m3 ? sc_context_e4m3 : sc_context_i8)(a, block_size, num_seqs, stream);
+  ScLaunch* launch = plan.tile_rows > 16 ? (plan.waves == 8 ? (e4m3 ? sc_context_e4m3_wide : sc_context_i8_wide)
+                                                            : (e4m3 ? sc_context_e4m3 : sc_context_i8))
+                                         : (plan.waves == 8 ? (e4m3 ? sc_decode_e4m3_wide : sc_decode_i8_wide)
+                                                            : (e4m3 ? sc_decode_e4m3 : sc_decode_i8));
+  const int rc = launch(a, block_size, num_seqs, stream);
   if (rc != SW_OK || num_parts == 1) return rc;
-  const dim3 grid(max_new_len, a.heads, num_seqs);
-  const int threads = (a.head_size + 63) / 64 * 64;
-  if (block_size == 8) scaled_join_kernel<8><<<grid, threads, 0, stream>>>(a);
-  else if (block_size == 16) scaled_join_kernel<16><<<grid, threads, 0, stream>>>(a);
-  else scaled_join_kernel<32><<<grid, threads, 0, stream>>>(a);
+  (block_size == 8 ? sc_join<8> : block_size == 16 ? sc_join<16> : sc_join<32>)(a, max_new_len, num_seqs, stream);
   SW_CHECK_LAUNCH();
   return SW_OK;
 }
@@ -114,11 +207,7 @@ extern "C" {
 
 int sw_scaled_attention_parts(int num_seqs, int max_new_len, int num_heads, int num_kv_heads, int head_size, int max_context_len) {
   if (num_seqs <= 0 || max_new_len <= 0 || num_kv_heads <= 0 || num_heads < num_kv_heads || max_context_len <= 0) return 1;
-  const int64_t rows = (int64_t)max_new_len * (num_heads / num_kv_heads), tile = sw::sc_tile_rows(rows);
-  const int64_t tiles = (rows + tile - 1) / tile;
-  const int64_t workgroups = (int64_t)num_seqs * num_kv_heads * tiles;
-  const int64_t most = ((int64_t)max_context_len + 255) / 256;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(most, 1024 / workgroups));
+  return sw::sc_plan(num_seqs, max_new_len, num_heads, num_kv_heads, head_size, max_context_len).parts;
 }
 
 int64_t sw_scaled_attention_workspace_bytes(int num_parts, int64_t num_rows, int num_heads, int head_size) {

@@ -1,6 +1,6 @@
 // Attention of many rows over the 8-bit cache with one scale for each (block, kv head) (included by scaled_context_*.hip).
 //
-// The mathematics of scaled_decode.cuh, for prompts: rows (new tokens times the query heads of a kv head) in tiles of 128, 32 a wave,
+// The mathematics of scaled_decode.cuh, for prompts: rows (new tokens times the query heads of a kv head) in tiles of 128 or 256, 32 a wave,
 // bound by the matrix products and the vector work beside them, 4 head_size operations a (row, token) on the one and some 8
 // instructions a (row, token) / 64 on the other.  So what can be done once for the workgroup is done once:
 //   * a stage of 64 tokens goes global -> registers (one stage ahead) -> halves -> LDS, where all waves read it as operands of
@@ -19,7 +19,7 @@ namespace sw {
 
 using sc_f32x16 = __attribute__((ext_vector_type(16))) float;
 
-constexpr int kScWaves = 4, kScRows = 32, kScTileRows = kScWaves * kScRows;
+constexpr int kScRows = 32;                                   // of a wave
 constexpr float kScLazy = 8.f;                                // powers of two by which a weight may pass 1
 constexpr float kScDeep = 40.f;                               // below the reference by more a value scale counts as that much below it
 
@@ -33,9 +33,10 @@ __host__ __device__ constexpr int sc_buffer(int head) {
   return sc_stage(head) * sc_kstride(head) + sc_padded(head) * sc_vstride(head) + 128;      // and the scales
 }
 
-template <bool E4M3, int HEAD, int BS>
-__global__ void __launch_bounds__(kScWaves * 64, 2) scaled_context_kernel(const ScAttention a) {
+template <bool E4M3, int HEAD, int BS, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScAttention a) {
   using C = ScCode<E4M3>;
+  constexpr int TILE = WAVES * kScRows;
   constexpr int KT = sc_stage(HEAD), NT = KT / 32, KS = HEAD / 16, DB = sc_padded(HEAD) / 32;
   constexpr int KSTRIDE = sc_kstride(HEAD), VSTRIDE = sc_vstride(HEAD), BUFFER = sc_buffer(HEAD);
   constexpr int PB = BS == 8 ? 2 : 1, SB = KT / 8;            // blocks of a run of 16 tokens; eights of a stage
@@ -49,10 +50,10 @@ __global__ void __launch_bounds__(kScWaves * 64, 2) scaled_context_kernel(const 
   const int tile = a.tiles - 1 - blockIdx.x / a.kv_heads, kv_head = blockIdx.x % a.kv_heads;
   const ScSequence s = sc_sequence<BS>(a, seq);
   const int rows = s.fresh * a.group;
-  if (tile * kScTileRows >= rows) return;
+  if (tile * TILE >= rows) return;
 
-  const int row0 = tile * kScTileRows;
-  const int pos_low = s.first + row0 / a.group, pos_high = s.first + min(rows - 1, row0 + kScTileRows - 1) / a.group;
+  const int row0 = tile * TILE;
+  const int pos_low = s.first + row0 / a.group, pos_high = s.first + min(rows - 1, row0 + TILE - 1) / a.group;
   const int begin = max(part * a.part_tokens, sc_seen_from(a, pos_low)), end = sc_part_end(a, s, part, pos_high);
   if (a.partial && begin >= end) return;                      // (the join knows)
 
@@ -111,7 +112,7 @@ __global__ void __launch_bounds__(kScWaves * 64, 2) scaled_context_kernel(const 
   const uint8_t* const v_base = a.value_cache + kv_head * head_bytes;
   const int32_t* table = a.tables + (int64_t)seq * a.table_stride;
   const int last_block = (s.len - 1) / BS;
-  constexpr int RUNS = KT / 16, SHARE = kScWaves / RUNS, NP = (HEAD + 64 * SHARE - 1) / (64 * SHARE);
+  constexpr int RUNS = KT / 16, SHARE = WAVES / RUNS, NP = (HEAD + 64 * SHARE - 1) / (64 * SHARE);
   const int run = wave / SHARE, u0 = (wave % SHARE) * 64 + lane;
   auto mine = [&](int i) { return HEAD % (64 * SHARE) == 0 || u0 + i * 64 * SHARE < HEAD; };
   // (stages behind the last one bring the last block again: what they lay down is not read)
@@ -238,29 +239,38 @@ __global__ void __launch_bounds__(kScWaves * 64, 2) scaled_context_kernel(const 
       for (int u = 0; u < NT; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[u][i] = 0.f;
-      // The scores' products, their operands read three ahead, and between them the next stage's widening: the order is held.
+      float fs[SB];
+#pragma unroll
+      for (int b = 0; b < SB; ++b) fs[b] = f[b] * row_scale;
+      auto top_of = [&](int b) {
+        const int u = b >> 2, i = (b & 3) * 4;
+        return fmaxf(fmaxf(x[u][i], x[u][i + 1]), fmaxf(x[u][i + 2], x[u][i + 3])) * fs[b];
+      };
+      float top = -INFINITY;
+      __builtin_amdgcn_s_setprio(1);
+      // The scores' products, their operands read three ahead; between them the next stage's widening and the maximum of the scores that
+      // are there: the order is held.
       {
-        auto operand = [&](int n) { return *reinterpret_cast<const sc_f16x8*>(kp + n % NT * 32 * KSTRIDE + n / NT * 32); };
+        auto operand = [&](int n) { return *reinterpret_cast<const sc_f16x8*>(kp + n / KS * 32 * KSTRIDE + n % KS * 32); };
         constexpr int N = NT * KS, AHEAD = 3, STEPS = kScSteps * NP;
         sc_f16x8 ring[AHEAD + 1];
 #pragma unroll
         for (int n = 0; n < AHEAD; ++n) ring[n] = operand(n);
         static_for<N>([&](auto I) {
-          constexpr int n = decltype(I)::value;
+          constexpr int n = decltype(I)::value, u = n / KS;
           if constexpr (n + AHEAD < N) ring[(n + AHEAD) % (AHEAD + 1)] = operand(n + AHEAD);
-          x[n % NT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[n % (AHEAD + 1)], __builtin_bit_cast(sc_f16x8, qf[n / NT]), x[n % NT], 0, 0, 0);
+          x[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[n % (AHEAD + 1)], __builtin_bit_cast(sc_f16x8, qf[n % KS]), x[u], 0, 0, 0);
           static_for<STEPS*(n + 1) / N - STEPS * n / N>(
               [&](auto K) { lay_step(std::integral_constant<int, STEPS * n / N + decltype(K)::value>{}, buf ^ 1); });
+          if constexpr (u > 0 && n % KS >= KS - 4) top = fmaxf(top, top_of(4 * u - 4 + n % KS - KS + 4));
           __builtin_amdgcn_sched_barrier(0);
         });
       }
+      __builtin_amdgcn_s_setprio(0);
       fetch(t0 + 2 * KT);
       look(t0 + 3 * KT);
 
-      // scores in powers of two: x fs (+ nothing more, where no row has anything to hide or to add)
-      float fs[SB];
-#pragma unroll
-      for (int b = 0; b < SB; ++b) fs[b] = f[b] * row_scale;
+      // scores in powers of two: x fs, where no row has anything to hide or to add
       const uint32_t missing = __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint32_t*>(f)[25]);
       const float ref = f[24];
       if (t0 + KT > wave_low + 1 || t0 < none_hidden || missing || a.slopes) {
@@ -276,13 +286,12 @@ __global__ void __launch_bounds__(kScWaves * 64, 2) scaled_context_kernel(const 
           }
 #pragma unroll
         for (int b = 0; b < SB; ++b) fs[b] = 1.f;
-      }
-      float top = -INFINITY;
+        top = -INFINITY;
 #pragma unroll
-      for (int b = 0; b < SB; ++b) {
-        const int u = b >> 2, i = (b & 3) * 4;
-        top = fmaxf(top, fmaxf(fmaxf(x[u][i], x[u][i + 1]), fmaxf(x[u][i + 2], x[u][i + 3])) * fs[b]);
+        for (int b = 0; b < SB - 4; ++b) top = fmaxf(top, top_of(b));
       }
+#pragma unroll
+      for (int b = SB - 4; b < SB; ++b) top = fmaxf(top, top_of(b));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       if (__any(top > m_run + kScLazy) || ref != ref_run) {
         const float m_new = fmaxf(m_run, top);
@@ -364,35 +373,35 @@ __global__ void __launch_bounds__(kScWaves * 64, 2) scaled_context_kernel(const 
     }
 }
 
-template <bool E4M3, int HEAD, int BS>
+template <bool E4M3, int HEAD, int BS, int WAVES>
 int sc_launch_context(const ScAttention& a, int num_seqs, hipStream_t stream) {
   constexpr int lds = 2 * sc_buffer(HEAD);
   static_assert(lds <= 160 * 1024, "two stages must fit a compute unit's LDS");
-  auto kernel = scaled_context_kernel<E4M3, HEAD, BS>;
+  auto kernel = scaled_context_kernel<E4M3, HEAD, BS, WAVES>;
   if (lds > 64 * 1024)
     SW_CHECK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-  kernel<<<dim3(a.kv_heads * a.tiles, num_seqs, a.parts), kScWaves * 64, lds, stream>>>(a);
+  kernel<<<dim3(a.kv_heads * a.tiles, num_seqs, a.parts), WAVES * 64, lds, stream>>>(a);
   SW_CHECK_LAUNCH();
   return SW_OK;
 }
 
-template <bool E4M3, int BS>
+template <bool E4M3, int BS, int WAVES>
 int sc_context_by_head(const ScAttention& a, int num_seqs, hipStream_t stream) {
   switch (a.head_size) {
-    case 64: return sc_launch_context<E4M3, 64, BS>(a, num_seqs, stream);
-    case 80: return sc_launch_context<E4M3, 80, BS>(a, num_seqs, stream);
-    case 96: return sc_launch_context<E4M3, 96, BS>(a, num_seqs, stream);
-    case 112: return sc_launch_context<E4M3, 112, BS>(a, num_seqs, stream);
-    case 128: return sc_launch_context<E4M3, 128, BS>(a, num_seqs, stream);
-    default: return sc_launch_context<E4M3, 256, BS>(a, num_seqs, stream);
+    case 64: return sc_launch_context<E4M3, 64, BS, WAVES>(a, num_seqs, stream);
+    case 80: return sc_launch_context<E4M3, 80, BS, WAVES>(a, num_seqs, stream);
+    case 96: return sc_launch_context<E4M3, 96, BS, WAVES>(a, num_seqs, stream);
+    case 112: return sc_launch_context<E4M3, 112, BS, WAVES>(a, num_seqs, stream);
+    case 128: return sc_launch_context<E4M3, 128, BS, WAVES>(a, num_seqs, stream);
+    default: return sc_launch_context<E4M3, 256, BS, WAVES>(a, num_seqs, stream);
   }
 }
 
-template <bool E4M3>
+template <bool E4M3, int WAVES>
 int sc_context_by_size(const ScAttention& a, int block_size, int num_seqs, hipStream_t stream) {
-  return block_size == 8    ? sc_context_by_head<E4M3, 8>(a, num_seqs, stream)
-         : block_size == 16 ? sc_context_by_head<E4M3, 16>(a, num_seqs, stream)
-                            : sc_context_by_head<E4M3, 32>(a, num_seqs, stream);
+  return block_size == 8    ? sc_context_by_head<E4M3, 8, WAVES>(a, num_seqs, stream)
+         : block_size == 16 ? sc_context_by_head<E4M3, 16, WAVES>(a, num_seqs, stream)
+                            : sc_context_by_head<E4M3, 32, WAVES>(a, num_seqs, stream);
 }
 
 }  // namespace sw

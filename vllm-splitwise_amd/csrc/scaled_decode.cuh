@@ -28,7 +28,7 @@ namespace sw {
 // NW waves take the groups of 64 tokens of one (sequence, kv head, tile of 16 rows, part) in turn and join at the end.
 // EXACT: head_size == HEAD; else it is a smaller multiple of 16 (dims behind it count as zeros).
 template <bool E4M3, int HEAD, bool EXACT, int BS, int NW>
-__global__ void __launch_bounds__(NW * 64) scaled_decode_kernel(const ScAttention a) {
+__global__ void __launch_bounds__(NW * 64, HEAD <= 128 ? 2 : 1) scaled_decode_kernel(const ScAttention a) {
   using C = ScCode<E4M3>;
   constexpr int KM = HEAD / 64, DT = HEAD / 16;
   constexpr int PB = BS == 8 ? 2 : 1;                        // blocks of a run of 16 tokens
@@ -38,7 +38,8 @@ __global__ void __launch_bounds__(NW * 64) scaled_decode_kernel(const ScAttentio
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r = lane & 15, kq = lane >> 4;
   const int seq = blockIdx.y, part = blockIdx.z;
-  const int kv_head = blockIdx.x / a.tiles, tile = blockIdx.x - kv_head * a.tiles;
+  // (all tiles of a kv head on one XCD where the number of heads is a multiple of 8)
+  const int tile = blockIdx.x / a.kv_heads, kv_head = blockIdx.x - tile * a.kv_heads;
   const ScSequence s = sc_sequence<BS>(a, seq);
   const int rows = s.fresh * a.group;
   if (tile * 16 >= rows) return;
@@ -161,13 +162,14 @@ __global__ void __launch_bounds__(NW * 64) scaled_decode_kernel(const ScAttentio
     sc_f32x4 x[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[j] = sc_f32x4{0.f, 0.f, 0.f, 0.f};
+    // (products into one accumulator lie four apart)
 #pragma unroll
     for (int m = 0; m < KM; ++m)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[j] = sc_mfma(sc_join(C::widen(kraw[j][m][0]), C::widen(kraw[j][m][1])), qf[m][0], x[j]);
-        x[j] = sc_mfma(sc_join(C::widen(kraw[j][m][2]), C::widen(kraw[j][m][3])), qf[m][1], x[j]);
-      }
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          x[j] = sc_mfma(sc_join(C::widen(kraw[j][m][2 * h]), C::widen(kraw[j][m][2 * h + 1])), qf[m][h], x[j]);
     const int run0 = tok0 + 16 * kq;
     const int left = end - run0;
     good &= left >= 16 ? 0xffffu : left <= 0 ? 0u : (1u << left) - 1u;
@@ -299,8 +301,8 @@ __global__ void __launch_bounds__(NW * 64) scaled_decode_kernel(const ScAttentio
 
 template <bool E4M3, int HEAD, bool EXACT, int BS, int NW>
 int sc_launch_decode(const ScAttention& a, int num_seqs, hipStream_t stream) {
-  const int lds = (NW * 32 + (NW / 2) * (HEAD / 16) * 256) * 4;
-  static_assert((NW * 32 + (NW / 2) * (HEAD / 16) * 256) * 4 <= 64 * 1024, "the waves' sums must fit a launch's plain LDS");
+  constexpr int lds = (NW * 32 + (NW / 2) * (HEAD / 16) * 256) * 4;
+  static_assert(lds <= 64 * 1024, "the waves' sums must fit a launch's plain LDS");
   scaled_decode_kernel<E4M3, HEAD, EXACT, BS, NW><<<dim3(a.kv_heads * a.tiles, num_seqs, a.parts), NW * 64, lds, stream>>>(a);
   SW_CHECK_LAUNCH();
   return SW_OK;
@@ -308,18 +310,20 @@ int sc_launch_decode(const ScAttention& a, int num_seqs, hipStream_t stream) {
 
 template <bool E4M3, int NW>
 int sc_decode_by_size(const ScAttention& a, int block_size, int num_seqs, hipStream_t stream) {
-  auto by_block = [&](auto head, auto exact) {
-    constexpr int H = decltype(head)::value;
+  auto by_block = [&](auto head, auto exact, auto waves) {
+    constexpr int H = decltype(head)::value, W = decltype(waves)::value;
     constexpr bool X = decltype(exact)::value;
-    return block_size == 8    ? sc_launch_decode<E4M3, H, X, 8, NW>(a, num_seqs, stream)
-           : block_size == 16 ? sc_launch_decode<E4M3, H, X, 16, NW>(a, num_seqs, stream)
-                              : sc_launch_decode<E4M3, H, X, 32, NW>(a, num_seqs, stream);
+    return block_size == 8    ? sc_launch_decode<E4M3, H, X, 8, W>(a, num_seqs, stream)
+           : block_size == 16 ? sc_launch_decode<E4M3, H, X, 16, W>(a, num_seqs, stream)
+                              : sc_launch_decode<E4M3, H, X, 32, W>(a, num_seqs, stream);
   };
+  const std::integral_constant<int, NW> waves{};
   switch (a.head_size) {
-    case 64: return by_block(std::integral_constant<int, 64>{}, std::true_type{});
-    case 128: return by_block(std::integral_constant<int, 128>{}, std::true_type{});
-    case 256: return by_block(std::integral_constant<int, 256>{}, std::true_type{});
-    default: return by_block(std::integral_constant<int, 128>{}, std::false_type{});
+    case 64: return by_block(std::integral_constant<int, 64>{}, std::true_type{}, waves);
+    case 128: return by_block(std::integral_constant<int, 128>{}, std::true_type{}, waves);
+    // (eight waves of such heads would have half the registers that they need)
+    case 256: return by_block(std::integral_constant<int, 256>{}, std::true_type{}, std::integral_constant<int, 4>{});
+    default: return by_block(std::integral_constant<int, 128>{}, std::false_type{}, waves);
   }
 }
 

@@ -4,4 +4,7 @@ namespace sw {
 int sc_decode_i8(const ScAttention& a, int block_size, int num_seqs, hipStream_t stream) {
   return sc_decode_by_size<false, 4>(a, block_size, num_seqs, stream);
 }
+int sc_decode_i8_wide(const ScAttention& a, int block_size, int num_seqs, hipStream_t stream) {
+  return sc_decode_by_size<false, 8>(a, block_size, num_seqs, stream);
+}
 }  // namespace sw
