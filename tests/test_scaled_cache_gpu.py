@@ -548,3 +548,44 @@ def test_blocks_copy_and_swap_like_any_cache():
     _C.cache_ops.swap_blocks(c.ks, host, {3: 0})
     torch.cuda.synchronize()
     assert torch.equal(host[0], c.ks[3].cpu())
+
+
+# --------------------------------------------------------------------------- the native side of small steps
+@pytest.mark.parametrize("kind", KINDS)
+def test_native_calls_do_the_same(kind, monkeypatch):
+    """Each operator through the native host side and through Python: the same bits, and the native side takes the plain call."""
+    from splitwise_amd import _native
+    if isinstance(_native.step_ops, _native._NotBuilt):
+        pytest.skip("_step_ops is not built")
+    lens, new = [700, 33], [3, 2]
+    tables = tables_for(lens, 16, 60).to(DEV)
+    i32 = [torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([0, 3], new, lens, [0, 700])]
+    query = random_query(5, 4, 64, torch.bfloat16)
+    x = random_query(5, 4, 64, torch.bfloat16, seed=1)
+    slots = slots_of(tables.cpu(), 16, [a - b for a, b in zip(lens, new)], new).to(DEV)
+    results = []
+    for native in (True, False):
+        answers = []
+
+        class Seen:
+            def __getattr__(self, name):
+                def run(*args):
+                    got = getattr(_native.step_ops, name)(*args) if native else None
+                    answers.append(got)
+                    return got
+                return run
+
+        monkeypatch.setattr(_C, "_native", Seen())
+        c = Cache(60, 2, 64, 16, kind)
+        _C.cache_ops.reshape_and_cache_scaled(x[:, :2], x[:, 2:], *c.device, slots, kind)
+        rows = [torch.zeros(733, 2, 64, dtype=torch.float16, device=DEV) for _ in range(2)]
+        _C.cache_ops.gather_cache_scaled(*rows, *c.device, tables, i32[3], i32[2], 700, kind)
+        one = torch.empty_like(query[:2])
+        _C.ops.paged_attention_scaled(one, query[:2], *c.device, 2, 0.1, tables, i32[2], 16, 700, None, kind)
+        few = torch.empty_like(query)
+        _C.ops.context_attention_scaled(few, query, *c.device, 0.1, tables, i32[0], i32[1], i32[2], 3, 700, None, kind, sliding_window=300)
+        assert answers == [0 if native else None] * 4
+        results.append([*c.device, *rows, one, few])
+        with pytest.raises(RuntimeError, match="heads must be contiguous"):
+            _C.ops.paged_attention_scaled(one, query[:2].transpose(1, 2), *c.device, 2, 0.1, tables, i32[2], 16, 700, None, kind)
+    assert all(torch.equal(a, b) for a, b in zip(*results))

@@ -28,7 +28,8 @@ namespace {
   X(swm_gated_delta_chunked) X(swm_gated_delta_chunked_workspace_floats) X(swm_head_norm_gate_act) X(swm_group_pairs)   \
   X(swm_expert_up_weighted) X(swm_expert_down_weighted) X(swm_masked_attention) X(swm_sink_attention)                   \
   X(swm_masked_attention_workspace_floats) X(swm_gla) X(swm_gla_workspace_floats) X(swm_lightning) X(swm_retention)     \
-  X(swm_lightning_workspace_floats)
+  X(swm_lightning_workspace_floats) X(sw_reshape_and_cache_scaled) X(sw_gather_cache_scaled) X(sw_paged_attention_scaled)  \
+  X(sw_context_attention_scaled) X(sw_scaled_attention_parts) X(sw_scaled_attention_workspace_bytes)
 // entry points of the libraries, set by bind() when one is loaded
 #define DECLARE(name) decltype(&::name) name##_at = nullptr;
 STEP_OPS(DECLARE)
@@ -317,6 +318,132 @@ STEP_OP(prefill_attention_and_cache) {
           (int)q.size(1), (int)k.size(1), (int)q.size(2), scale, nullptr, q.stride(0), k.stride(0), v.stride(0), out.stride(0), window,
           act, ptr<void>(kc), ptr<void>(vc), ptr<int64_t>(slots), (int)k.size(0), (int)kc.size(3), (int)kc.size(4), cache, stream);
     }));
+  });
+}
+
+// ------------------------------------------------------------- 8-bit cache with a scale for each (block, kv head)
+// What _scaled_caches checks.
+struct ScaledCache {
+  const Tensor &key, &value, &key_scales, &value_scales;
+  int type;
+  int64_t blocks, heads, size;
+  int block;
+  ScaledCache(const Args& c, int first, PyObject* name)
+      : key(c.tensor(first)), value(c.tensor(first + 1)), key_scales(c.tensor(first + 2)), value_scales(c.tensor(first + 3)) {
+    take(PyUnicode_Check(name));
+    const bool e4m3 = PyUnicode_CompareWithASCIIString(name, "fp8_e4m3") == 0;
+    take(e4m3 || PyUnicode_CompareWithASCIIString(name, "int8") == 0);
+    type = e4m3 ? SW_E4M3_SCALED : SW_I8_SCALED;
+    take(key.dim() == 5 && value.dim() == 4 && key.scalar_type() == at::kByte && value.scalar_type() == at::kByte);
+    blocks = value.size(0), heads = value.size(1), size = value.size(2), block = (int)value.size(3);
+    take(key.size(0) == blocks && key.size(1) == heads && key.size(2) == size / 16 && key.size(3) == block && key.size(4) == 16);
+    for (const Tensor* t : {&key_scales, &value_scales}) {
+      f32c(*t);
+      take(is(*t, blocks, heads));
+    }
+    take(key.is_contiguous() && value.is_contiguous());
+  }
+};
+// _scaled_rows of a tensor and another one of its shape and type
+void scaled_rows(const Tensor& a, const Tensor& b) {
+  take(a.dim() == 3 && b.dim() == 3 && a.sizes() == b.sizes() && a.scalar_type() == b.scalar_type());
+  for (const Tensor* t : {&a, &b}) take(t->numel() == 0 || (t->stride(2) == 1 && t->stride(1) == t->size(2)));
+  take(a.size(0) <= INT32_MAX);
+}
+void scaled_table(const Tensor& tables, std::initializer_list<const Tensor*> lengths) {
+  take(tables.dim() == 2 && tables.scalar_type() == at::kInt && (tables.numel() == 0 || tables.stride(1) == 1) && tables.size(0) <= INT32_MAX);
+  for (const Tensor* t : lengths) take(t->dim() == 1 && t->scalar_type() == at::kInt && t->is_contiguous() && t->size(0) == tables.size(0));
+}
+
+STEP_OP(reshape_and_cache_scaled) {
+  return call([&] {
+    const Args c(args, nargs, 8);
+    take(sw_reshape_and_cache_scaled_at != nullptr);
+    const Tensor &key = c.tensor(0), &value = c.tensor(1), &slots = c.tensor(6);
+    const ScaledCache k(c, 2, args[7]);
+    scaled_rows(key, value);
+    const int act = hip_act(key);
+    take(key.size(1) == k.heads && key.size(2) == k.size && slots.scalar_type() == at::kLong && slots.dim() == 1
+         && slots.size(0) == key.size(0) && slots.is_contiguous());
+    void* stream = c.stream();
+    return PyLong_FromLong(unlocked([&] {
+      return sw_reshape_and_cache_scaled_at(ptr<void>(key), ptr<void>(value), ptr<void>(k.key), ptr<void>(k.value), ptr(k.key_scales),
+                                            ptr(k.value_scales), ptr<int64_t>(slots), (int)key.size(0), (int)k.heads, (int)k.size,
+                                            k.block, k.blocks, key.stride(0), value.stride(0), act, k.type, stream);
+    }));
+  });
+}
+
+STEP_OP(gather_cache_scaled) {
+  return call([&] {
+    const Args c(args, nargs, 11);
+    take(sw_gather_cache_scaled_at != nullptr);
+    const Tensor &key = c.tensor(0), &value = c.tensor(1), &tables = c.tensor(6), &starts = c.tensor(7), &lens = c.tensor(8);
+    const ScaledCache k(c, 2, args[10]);
+    const int longest = c.i32(9);
+    scaled_rows(key, value);
+    scaled_table(tables, {&starts, &lens});
+    const int act = hip_act(key);
+    take(key.size(1) == k.heads && key.size(2) == k.size);
+    void* stream = c.stream();
+    return PyLong_FromLong(unlocked([&] {
+      return sw_gather_cache_scaled_at(ptr<void>(key), ptr<void>(value), ptr<void>(k.key), ptr<void>(k.value), ptr(k.key_scales),
+                                       ptr(k.value_scales), ptr<int32_t>(tables), ptr<int32_t>(starts), ptr<int32_t>(lens),
+                                       (int)lens.size(0), longest, key.size(0), (int)k.heads, (int)k.size, k.block, k.blocks,
+                                       (int)tables.size(1), tables.stride(0), key.stride(0), value.stride(0), act, k.type, stream);
+    }));
+  });
+}
+
+// Both attentions.  starts null: one new token a sequence.
+PyObject* scaled_attention(const Args& c, const ScaledCache& k, int kv_heads, float scale, const Tensor& tables, const Tensor* starts,
+                           const Tensor* fresh, const Tensor& lens, int most_new, int longest, int window) {
+  const Tensor &out = c.tensor(0), &query = c.tensor(1);
+  scaled_rows(query, out);
+  const int act = hip_act(query);
+  take(act != SW_F32 && query.size(2) == k.size && kv_heads == k.heads);
+  const int64_t rows = query.size(0);
+  const int heads = (int)query.size(1), seqs = (int)lens.size(0);
+  const int parts = sw_scaled_attention_parts_at(seqs, most_new, heads, kv_heads, (int)k.size, longest);
+  const int64_t need = sw_scaled_attention_workspace_bytes_at(parts, rows, heads, (int)k.size);
+  const Tensor work = need > 0 ? at::empty({need}, query.options().dtype(at::kByte)) : Tensor();
+  void* scratch = need > 0 ? ptr<void>(work) : nullptr;
+  void* stream = c.stream();
+  return PyLong_FromLong(unlocked([&] {
+    if (starts == nullptr)
+      return sw_paged_attention_scaled_at(ptr<void>(out), ptr<void>(query), ptr<void>(k.key), ptr<void>(k.value), ptr(k.key_scales),
+                                          ptr(k.value_scales), seqs, heads, kv_heads, (int)k.size, scale, ptr<int32_t>(tables),
+                                          ptr<int32_t>(lens), k.block, k.blocks, longest, (int)tables.size(1), tables.stride(0), nullptr,
+                                          query.stride(0), out.stride(0), act, k.type, parts, scratch, need, stream);
+    return sw_context_attention_scaled_at(ptr<void>(out), ptr<void>(query), ptr<void>(k.key), ptr<void>(k.value), ptr(k.key_scales),
+                                          ptr(k.value_scales), seqs, rows, heads, kv_heads, (int)k.size, scale, ptr<int32_t>(tables),
+                                          ptr<int32_t>(*starts), ptr<int32_t>(*fresh), ptr<int32_t>(lens), k.block, k.blocks, most_new,
+                                          longest, (int)tables.size(1), tables.stride(0), nullptr, window, query.stride(0), out.stride(0),
+                                          act, k.type, parts, scratch, need, stream);
+  }));
+}
+
+STEP_OP(paged_attention_scaled) {
+  return call([&] {
+    const Args c(args, nargs, 13);
+    take(sw_paged_attention_scaled_at != nullptr);
+    const Tensor &query = c.tensor(1), &tables = c.tensor(8), &lens = c.tensor(9);
+    const ScaledCache k(c, 2, args[12]);
+    scaled_table(tables, {&lens});
+    take(query.dim() == 3 && query.size(0) == tables.size(0) && c.i32(10) == k.block);
+    return scaled_attention(c, k, c.i32(6), c.f32(7), tables, nullptr, nullptr, lens, 1, c.i32(11), 0);
+  });
+}
+
+STEP_OP(context_attention_scaled) {
+  return call([&] {
+    const Args c(args, nargs, 15);
+    take(sw_context_attention_scaled_at != nullptr);
+    const Tensor &tables = c.tensor(7), &starts = c.tensor(8), &fresh = c.tensor(9), &lens = c.tensor(10);
+    const ScaledCache k(c, 2, args[13]);
+    scaled_table(tables, {&starts, &fresh, &lens});
+    return scaled_attention(c, k, (int)k.heads, c.f32(6), tables, &starts, &fresh, lens, c.i32(11), c.i32(12),
+                            args[14] == Py_None ? 0 : c.i32(14));
   });
 }
 
@@ -621,6 +748,7 @@ PyObject* bind(PyObject*, PyObject* table) {
 PyMethodDef kMethods[] = {
     METHOD(reshape_and_cache) METHOD(paged_attention_v1) METHOD(prefill_attention) METHOD(causal_conv) METHOD(gated_delta)
     METHOD(prefill_attention_and_cache) METHOD(paged_attention_and_cache)
+    METHOD(reshape_and_cache_scaled) METHOD(gather_cache_scaled) METHOD(paged_attention_scaled) METHOD(context_attention_scaled)
     METHOD(head_norm_gate) METHOD(gla) METHOD(lightning) METHOD(retention) METHOD(group_pairs) METHOD(expert_ffn)
     METHOD(capped_attention) {"bind", bind, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -44,13 +44,14 @@ __device__ __forceinline__ ScSequence sc_sequence(const ScAttention& a, int seq)
 __device__ __forceinline__ float sc_from16(uint32_t half, bool bf16) {
   return bf16 ? bf16_bits_to_float((uint16_t)half) : f16_bits_to_float((uint16_t)half);
 }
-__device__ __forceinline__ uint32_t sc_pack16(float a, float b, bool bf16) {
-  return bf16 ? (uint32_t)float_to_bf16_bits(a) | ((uint32_t)float_to_bf16_bits(b) << 16)
-              : (uint32_t)float_to_f16_bits(a) | ((uint32_t)float_to_f16_bits(b) << 16);
-}
 __device__ __forceinline__ uint32_t sc_pack_f16(float a, float b) {
   using f32x2 = __attribute__((ext_vector_type(2))) float;
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), sc_f16x2));     // one instruction, to the nearest
+}
+__device__ __forceinline__ uint32_t sc_pack16(float a, float b, bool bf16) {
+  using f32x2 = __attribute__((ext_vector_type(2))) float;
+  using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
+  return bf16 ? __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2)) : sc_pack_f16(a, b);
 }
 
 __device__ __forceinline__ sc_f32x4 sc_mfma(sc_u32x4 a, sc_u32x4 b, sc_f32x4 c) {

@@ -24,6 +24,13 @@ template <> struct ScCode<false> {
   __device__ static __forceinline__ uint32_t encode(float a, float b, float c, float d) {
     return byte(a) | (byte(b) << 8) | (byte(c) << 16) | (byte(d) << 24);
   }
+  // the same of finite values that a scale of theirs has brought to +-127: 1.5 x 2^23 + v has v's nearest integer in its low byte
+  __device__ static __forceinline__ uint32_t encode_fitting(float a, float b, float c, float d, float inverse) {
+    constexpr float at = 12582912.f;
+    const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(fmaf(b, inverse, at)), __float_as_uint(fmaf(a, inverse, at)), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(fmaf(d, inverse, at)), __float_as_uint(fmaf(c, inverse, at)), 0x04000c0cu);
+    return lo | hi;
+  }
   __device__ static __forceinline__ uint32_t byte(float x) {
     const float y = rintf(__builtin_amdgcn_fmed3f(x, -kTop, kTop));
     return (uint32_t)(int)(x != x ? 0.f : y) & 0xffu;
@@ -33,6 +40,15 @@ template <> struct ScCode<false> {
     o[1] = (float)(int)(int8_t)((w >> 8) & 0xffu);
     o[2] = (float)(int)(int8_t)((w >> 16) & 0xffu);
     o[3] = (float)((int)w >> 24);
+  }
+  // four codes times a scale, each rounded once: (code + 128) scale - 128 scale in one operation
+  __device__ static __forceinline__ void scaled(uint32_t w, float scale, float* o) {
+    const uint32_t u = w ^ 0x80808080u;
+    const float off = -128.f * scale;
+    o[0] = fmaf((float)(u & 0xffu), scale, off);
+    o[1] = fmaf((float)((u >> 8) & 0xffu), scale, off);
+    o[2] = fmaf((float)((u >> 16) & 0xffu), scale, off);
+    o[3] = fmaf((float)(u >> 24), scale, off);
   }
   // four codes as four halves, exactly: 0x6400 | u is 1024 + u, u = code + 128
   __device__ static __forceinline__ sc_u32x2 widen(uint32_t w) {
@@ -62,6 +78,17 @@ template <> struct ScCode<true> {
     o[1] = lo[1];
     o[2] = hi[0];
     o[3] = hi[1];
+  }
+  // (the conversion takes what is a rounding above 448 to 448)
+  __device__ static __forceinline__ uint32_t encode_fitting(float a, float b, float c, float d, float inverse) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a * inverse, b * inverse, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(c * inverse, d * inverse, w, true);
+    return (uint32_t)w;
+  }
+  __device__ static __forceinline__ void scaled(uint32_t w, float scale, float* o) {
+    decode(w, o);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] *= scale;
   }
   // (e4m3's 4 bits of magnitude and powers down to 2^-9 fit a half exactly)
   __device__ static __forceinline__ sc_u32x2 widen(uint32_t w) {

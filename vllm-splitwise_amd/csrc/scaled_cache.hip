@@ -26,7 +26,7 @@ struct ScWrite {
   const int64_t* slots;
   int64_t stride[2];           // elements from token to token
   int64_t num_slots;           // blocks * block size
-  int num_tokens, heads, head_size, window;
+  int num_tokens, heads, head_size, window, head_pairs;
 };
 
 struct ScRead {
@@ -35,12 +35,13 @@ struct ScRead {
   const float* scales[2];
   const int32_t *tables, *starts, *lens;
   int64_t stride[2], num_rows, table_stride;
-  int num_blocks, width, heads, head_size;
+  int num_blocks, width, heads, head_size, head_pairs;
 };
 
 template <typename act_t> struct ScAct {
   using S = typename Conv<act_t>::store_t;
   static constexpr int kWords = sizeof(S) * 16 / 4;            // dwords of 16 elements
+  static constexpr uint32_t kInf = std::is_same<act_t, f16_t>::value ? 0x7c00u : std::is_same<act_t, bf16_t>::value ? 0x7f80u : 0x7f800000u;
   // element `i` of the dwords at w
   __device__ static __forceinline__ float get(const uint32_t* w, int i) {
     if constexpr (sizeof(S) == 4) return __uint_as_float(w[i]);
@@ -48,13 +49,46 @@ template <typename act_t> struct ScAct {
   }
   __device__ static __forceinline__ uint32_t pair(float a, float b) {
     static_assert(sizeof(S) == 2 || sizeof(S) == 4, "");
-    return (uint32_t)Conv<act_t>::from_float(a) | ((uint32_t)Conv<act_t>::from_float(b) << 16);
+    using f32x2 = __attribute__((ext_vector_type(2))) float;
+    using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
+    if constexpr (std::is_same<act_t, f16_t>::value) return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), sc_f16x2));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
   }
+  // Magnitudes are compared as the integers that their bits are (16-bit ones two at a time): infinities and NaN are the largest.
+  using u16x2 = __attribute__((ext_vector_type(2))) uint16_t;
+  __device__ static __forceinline__ void larger(uint32_t& most, uint32_t w) {
+    if constexpr (sizeof(S) == 4) most = max(most, w & 0x7fffffffu);
+    else most = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, most), __builtin_bit_cast(u16x2, w & 0x7fff7fffu)));
+  }
+  // a wave's largest magnitude, as its bits
+  __device__ static __forceinline__ uint32_t largest(uint32_t most) {
+    if constexpr (sizeof(S) == 2) most = max(most & 0xffffu, most >> 16);
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) most = max(most, (uint32_t)__shfl_xor((int)most, m, 64));
+    return __builtin_amdgcn_readfirstlane(most);
+  }
+  __device__ static __forceinline__ float value(uint32_t bits) { return get(&bits, 0); }
 };
 
 __device__ __forceinline__ float sc_magnitude(float x) {
   const float a = fabsf(x);
   return a < INFINITY ? a : 0.f;                               // neither infinities nor NaN count
+}
+
+// Of four lanes 16 apart, r[k] of lane q becomes r[q] of lane k: two swaps of halves, two of 16 lanes.
+__device__ __forceinline__ void sc_transpose(uint32_t (&r)[4]) {
+  auto swap32 = [](uint32_t& a, uint32_t& b) {
+    const auto t = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = t[0], b = t[1];
+  };
+  auto swap16 = [](uint32_t& a, uint32_t& b) {
+    const auto t = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    a = t[0], b = t[1];
+  };
+  swap32(r[0], r[2]);
+  swap32(r[1], r[3]);
+  swap16(r[0], r[1]);
+  swap16(r[2], r[3]);
 }
 
 struct ScScale { float now, inverse, ratio; };
@@ -75,57 +109,74 @@ __device__ __forceinline__ uint32_t sc_rescale(uint32_t w, float ratio) {
   return ScCode<E4M3>::encode(o[0] * ratio, o[1] * ratio, o[2] * ratio, o[3] * ratio);
 }
 
-// token of the call that goes to offset o of the block, -1: none
-struct ScTokens {
-  const int* map;              // LDS, or null: first + o
-  int first;
-  __device__ __forceinline__ int operator()(int o) const { return map ? map[o] : first + o; }
-};
+constexpr int kScWindow = 16;        // entries of a workgroup; they, one before them and a block behind them are a wave's lanes
+constexpr int kScLook = 16;          // entries that a thread asks for at a time as it goes through the list
 
-// A lane's pieces are 16 elements of one token's key: 32 bytes in, one 16-byte store.
-template <typename act_t, bool E4M3, int BS, int DMAX>
-__device__ __forceinline__ void sc_write_keys(const ScWrite& w, int64_t block, int head, const ScTokens& token, int lane) {
+// Bound by vector instructions as much as by memory (an element is 2 bytes in and 1 out), so: a lane's addresses are one number and what
+// the compiler can put into the instructions; magnitudes two at a time; codes of finite values, the rule, in 3 instructions an element; and
+// blocks that the call fills look at no single token.
+
+// A lane's pieces are 16 elements of the key of one token, the same for all its pieces: 32 bytes in (64 of fp32), 16 out, where a wave's lie
+// side by side.  FULL: tokens first, first + 1, ... fill the block.
+template <typename act_t, bool E4M3, int BS, int DMAX, bool FULL>
+__device__ __forceinline__ void sc_write_keys(const ScWrite& w, int64_t block, int head, const int* map, int first, int lane) {
   using A = ScAct<act_t>;
-  constexpr int NU = (BS * DMAX / 16 + 63) / 64;
-  const int chunks = w.head_size >> 4, units = BS * chunks;
+  constexpr int NU = (BS * DMAX / 16 + 63) / 64, STEP = 64 / BS;
+  const int chunks = w.head_size >> 4, t = lane % BS, c0 = lane / BS;
   const int64_t bh = block * w.heads + head;
-  uint8_t* out = w.cache[0] + bh * w.head_size * BS;
+  uint8_t* out = w.cache[0] + bh * w.head_size * BS + lane * 16;
   const float stored = w.scales[0][bh];
-  uint32_t x[NU][A::kWords];
-  int tok[NU], at[NU];
-  float largest = 0.f;
+  const int tok = FULL ? first + t : map[t];
+  const typename A::S* in = reinterpret_cast<const typename A::S*>(w.x[0]) + tok * w.stride[0] + (int64_t)head * w.head_size + 16 * c0;
+  uint32_t x[NU][A::kWords], most = 0;
 #pragma unroll
   for (int i = 0; i < NU; ++i) {
-    const int u = lane + 64 * i, t = u / chunks, c = u - t * chunks;
-    tok[i] = u < units ? token(t) : -1;
-    at[i] = u < units ? (c * BS + t) * 16 : -1;
-    if (tok[i] >= 0) {
-      const sc_u32x4* p = reinterpret_cast<const sc_u32x4*>(reinterpret_cast<const typename A::S*>(w.x[0]) + tok[i] * w.stride[0] +
-                                                            (int64_t)head * w.head_size + 16 * c);
 #pragma unroll
-      for (int k = 0; k < A::kWords / 4; ++k) *reinterpret_cast<sc_u32x4*>(&x[i][4 * k]) = p[k];
+    for (int k = 0; k < A::kWords; ++k) x[i][k] = 0;
+    if (c0 + i * STEP < chunks && (FULL || tok >= 0)) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) largest = fmaxf(largest, sc_magnitude(A::get(x[i], e)));
+      for (int k = 0; k < A::kWords / 4; ++k)
+        *reinterpret_cast<sc_u32x4*>(&x[i][4 * k]) = reinterpret_cast<const sc_u32x4*>(in + 16 * STEP * i)[k];
     }
   }
-  const bool fresh = token(0) >= 0;
-  const ScScale s = sc_scale<E4M3>(wave_max(largest), fresh ? 0.f : sc_old_scale(stored));
+#pragma unroll
+  for (int i = 0; i < NU; ++i)
+#pragma unroll
+    for (int k = 0; k < A::kWords; ++k) A::larger(most, x[i][k]);
+  most = A::largest(most);
+  const bool finite = most < A::kInf;
+  float largest = A::value(most);
+  if (!finite) {
+    largest = 0.f;
+#pragma unroll
+    for (int i = 0; i < NU; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) largest = fmaxf(largest, sc_magnitude(A::get(x[i], e)));
+    largest = wave_max(largest);
+  }
+  const bool fresh = FULL || map[0] >= 0;
+  const ScScale s = sc_scale<E4M3>(largest, fresh ? 0.f : sc_old_scale(stored));
   if (lane == 0) w.scales[0][bh] = s.now;
 #pragma unroll
   for (int i = 0; i < NU; ++i) {
-    if (at[i] < 0) continue;
-    sc_u32x4* p = reinterpret_cast<sc_u32x4*>(out + at[i]);
-    if (tok[i] >= 0) {
-      sc_u32x4 q;
+    if (c0 + i * STEP >= chunks) continue;
+    sc_u32x4* p = reinterpret_cast<sc_u32x4*>(out + i * 64 * 16);
+    sc_u32x4 q;
+    if (finite) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        q[k] = ScCode<E4M3>::encode_fitting(A::get(x[i], 4 * k), A::get(x[i], 4 * k + 1), A::get(x[i], 4 * k + 2), A::get(x[i], 4 * k + 3),
+                                            s.inverse);
+    } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         q[k] = ScCode<E4M3>::encode(A::get(x[i], 4 * k) * s.inverse, A::get(x[i], 4 * k + 1) * s.inverse,
                                     A::get(x[i], 4 * k + 2) * s.inverse, A::get(x[i], 4 * k + 3) * s.inverse);
+    }
+    if (FULL || tok >= 0 || fresh) {                           // (slots without a token are zeros: x is)
       *p = q;
-    } else if (fresh) {
-      *p = sc_u32x4{0u, 0u, 0u, 0u};
     } else if (s.ratio != 1.f) {
-      sc_u32x4 q = *p;
+      q = *p;
 #pragma unroll
       for (int k = 0; k < 4; ++k) q[k] = sc_rescale<E4M3>(q[k], s.ratio);
       *p = q;
@@ -133,34 +184,33 @@ __device__ __forceinline__ void sc_write_keys(const ScWrite& w, int64_t block, i
   }
 }
 
-// A lane's pieces are two elements of every token's value: 4 bytes a token in (a wave's load is a whole row of 128), two rows of the
-// block's tokens out, 2 * BS bytes side by side.
-template <typename act_t, bool E4M3, int BS, int DMAX>
-__device__ __forceinline__ void sc_write_values(const ScWrite& w, int64_t block, int head, const ScTokens& token, int lane) {
+// A lane's pieces are two elements of every token's value: 4 bytes a token in (a wave's load is a whole row of 128, where the token's row
+// begins is a scalar), two rows of the block's tokens out, 2 * BS bytes side by side.
+template <typename act_t, bool E4M3, int BS, int DMAX, bool FULL>
+__device__ __forceinline__ void sc_write_values(const ScWrite& w, int64_t block, int head, const int* map, int first, int lane) {
   using A = ScAct<act_t>;
-  constexpr int NP = DMAX / 128, W2 = sizeof(typename A::S) / 2;      // W2: dwords of two elements
+  using S = typename A::S;
+  constexpr int NP = DMAX / 128, W2 = sizeof(S) / 2;                   // W2: dwords of two elements
   const int pairs = w.head_size >> 1;
   const int64_t bh = block * w.heads + head;
   uint8_t* out = w.cache[1] + bh * w.head_size * BS;
   const float stored = w.scales[1][bh];
-  uint32_t x[NP][BS][W2];
-  float largest = 0.f;
+  const S* in = reinterpret_cast<const S*>(w.x[1]) + (int64_t)head * w.head_size;
+  uint32_t x[NP][BS][W2], most = 0;
   uint32_t there = 0;                                                   // bit o: a token goes to offset o
 #pragma unroll
-  for (int o = 0; o < BS; ++o) there |= (token(o) >= 0 ? 1u : 0u) << o;
-  there = __builtin_amdgcn_readfirstlane(there);
+  for (int o = 0; o < BS; ++o) {
+    const int tok = FULL ? first + o : __builtin_amdgcn_readfirstlane(map[o]);
+    there |= (FULL || tok >= 0 ? 1u : 0u) << o;
+    const char* row = reinterpret_cast<const char*>(in + tok * w.stride[1]);
 #pragma unroll
-  for (int i = 0; i < NP; ++i) {
-    const int p = lane + 64 * i;
-#pragma unroll
-    for (int o = 0; o < BS; ++o) {
+    for (int i = 0; i < NP; ++i) {
+      const uint32_t p = lane + 64 * i;
 #pragma unroll
       for (int k = 0; k < W2; ++k) x[i][o][k] = 0;
-      if ((there >> o & 1u) && p < pairs) {
-        const typename A::S* src = reinterpret_cast<const typename A::S*>(w.x[1]) + token(o) * w.stride[1] +
-                                   (int64_t)head * w.head_size + 2 * p;
-        if constexpr (W2 == 1) x[i][o][0] = *reinterpret_cast<const uint32_t*>(src);
-        else *reinterpret_cast<sc_u32x2*>(x[i][o]) = *reinterpret_cast<const sc_u32x2*>(src);
+      if ((FULL || tok >= 0) && (int)p < pairs) {
+        if constexpr (W2 == 1) x[i][o][0] = *reinterpret_cast<const uint32_t*>(row + p * 4);
+        else *reinterpret_cast<sc_u32x2*>(x[i][o]) = *reinterpret_cast<const sc_u32x2*>(row + p * 8);
       }
     }
   }
@@ -168,33 +218,51 @@ __device__ __forceinline__ void sc_write_values(const ScWrite& w, int64_t block,
   for (int i = 0; i < NP; ++i)
 #pragma unroll
     for (int o = 0; o < BS; ++o)
-      largest = fmaxf(largest, fmaxf(sc_magnitude(A::get(x[i][o], 0)), sc_magnitude(A::get(x[i][o], 1))));
+#pragma unroll
+      for (int k = 0; k < W2; ++k) A::larger(most, x[i][o][k]);
+  most = A::largest(most);
+  const bool finite = most < A::kInf;
+  float largest = A::value(most);
+  if (!finite) {
+    largest = 0.f;
+#pragma unroll
+    for (int i = 0; i < NP; ++i)
+#pragma unroll
+      for (int o = 0; o < BS; ++o)
+        largest = fmaxf(largest, fmaxf(sc_magnitude(A::get(x[i][o], 0)), sc_magnitude(A::get(x[i][o], 1))));
+    largest = wave_max(largest);
+  }
   const bool fresh = there & 1u;
-  const ScScale s = sc_scale<E4M3>(wave_max(largest), fresh ? 0.f : sc_old_scale(stored));
+  const ScScale s = sc_scale<E4M3>(largest, fresh ? 0.f : sc_old_scale(stored));
   if (lane == 0) w.scales[1][bh] = s.now;
-  const bool merge = !fresh && there != (BS == 32 ? 0xffffffffu : (1u << (BS & 31)) - 1u);
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     const int p = lane + 64 * i;
     if (p >= pairs) continue;
-    uint32_t* row = reinterpret_cast<uint32_t*>(out + (int64_t)2 * p * BS);
+    uint32_t* row = reinterpret_cast<uint32_t*>(out + (uint32_t)(2 * p * BS));
     uint32_t q[2][BS / 4];
 #pragma unroll
     for (int e = 0; e < 2; ++e)
 #pragma unroll
       for (int k = 0; k < BS / 4; ++k) {
-        const uint32_t some = there >> (4 * k) & 15u;
-        uint32_t was = 0;
-        if (merge && some != 15u) {
-          was = row[e * (BS / 4) + k];
-          if (s.ratio != 1.f) was = sc_rescale<E4M3>(was, s.ratio);
-        }
-        const uint32_t now = ScCode<E4M3>::encode(A::get(x[i][4 * k], e) * s.inverse, A::get(x[i][4 * k + 1], e) * s.inverse,
-                                                  A::get(x[i][4 * k + 2], e) * s.inverse, A::get(x[i][4 * k + 3], e) * s.inverse);
-        const uint32_t mask = (some & 1u ? 0xffu : 0u) | (some & 2u ? 0xff00u : 0u) | (some & 4u ? 0xff0000u : 0u) |
-                              (some & 8u ? 0xff000000u : 0u);
-        q[e][k] = (now & mask) | (was & ~mask);
+        const float v0 = A::get(x[i][4 * k], e), v1 = A::get(x[i][4 * k + 1], e), v2 = A::get(x[i][4 * k + 2], e), v3 = A::get(x[i][4 * k + 3], e);
+        q[e][k] = finite ? ScCode<E4M3>::encode_fitting(v0, v1, v2, v3, s.inverse)
+                         : ScCode<E4M3>::encode(v0 * s.inverse, v1 * s.inverse, v2 * s.inverse, v3 * s.inverse);
       }
+    if (!FULL && !fresh) {                                      // what the call does not write is kept
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int k = 0; k < BS / 4; ++k) {
+          const uint32_t some = there >> (4 * k) & 15u;
+          if (some == 15u) continue;
+          uint32_t was = row[e * (BS / 4) + k];
+          if (s.ratio != 1.f) was = sc_rescale<E4M3>(was, s.ratio);
+          const uint32_t mask = (some & 1u ? 0xffu : 0u) | (some & 2u ? 0xff00u : 0u) | (some & 4u ? 0xff0000u : 0u) |
+                                (some & 8u ? 0xff000000u : 0u);
+          q[e][k] = (q[e][k] & mask) | (was & ~mask);
+        }
+    }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       if constexpr (BS >= 16) {
@@ -212,63 +280,75 @@ template <typename act_t, bool E4M3, int BS, int DMAX>
 __global__ void __launch_bounds__(256) scaled_write_kernel(const ScWrite w) {
   __shared__ int map[BS], earlier;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int head = blockIdx.y * 2 + (wave >> 1);
-  const int t0 = blockIdx.x * w.window;
+  // (all heads of a stretch of the list side by side in time: a token's row, and a block, are whole then)
+  const int stretch = blockIdx.x / w.head_pairs, head = (blockIdx.x - stretch * w.head_pairs) * 2 + (wave >> 1);
+  const int t0 = stretch * w.window;
   auto block_of = [&](int64_t slot) -> int64_t { return slot >= 0 && slot < w.num_slots ? slot / BS : -1; };
-  auto slot_of = [&](int t) -> int64_t { return t < w.num_tokens ? w.slots[t] : -1; };
+  auto slot_of = [&](int t) -> int64_t { return t >= 0 && t < w.num_tokens ? w.slots[t] : -1; };
 
-  // heads of runs among this workgroup's entries (every wave finds the same ones)
-  uint64_t heads;
-  {
-    const int t = t0 + lane;
-    const int64_t mine = lane < w.window ? block_of(slot_of(t)) : -1;
-    const int64_t before = lane < w.window && t > 0 ? block_of(slot_of(t - 1)) : -1;
-    heads = __ballot(mine >= 0 && mine != before);
-  }
+  // lane l: entry t0 - 1 + l (its block), of which `window` are this workgroup's; those whose predecessor is in another block are heads
+  // of runs (every wave finds the same ones)
+  const int64_t near = slot_of(t0 - 1 + lane), near_block = block_of(near), before = __shfl_up(near_block, 1, 64);
+  uint64_t heads = __ballot(lane >= 1 && lane <= w.window && near_block >= 0 && near_block != before);
   while (heads) {
-    const int t = t0 + __builtin_ctzll(heads);
+    const int at = __builtin_ctzll(heads), t = t0 - 1 + at;
     heads &= heads - 1;
-    const int64_t first = w.slots[t], block = first / BS;
-    // the whole block in order, and nothing of it right behind
-    const int64_t next = lane <= BS ? slot_of(t + lane) : -1;
-    const bool as_run = lane < BS ? next == first + lane : lane > BS || block_of(next) != block;
-    ScTokens token{nullptr, t};
-    if (first % BS != 0 || __ballot(as_run) != ~0ull) {
+    const int64_t first = __shfl(near, at, 64), block = first / BS;
+    // the whole block in order, and nothing of it right behind (a window and a block behind it are lanes of the wave)
+    const bool as_run = lane < at || lane > at + BS || (lane < at + BS ? near == first + (lane - at) : near_block != block);
+    const bool full = first % BS == 0 && __ballot(as_run) == ~0ull;
+    if (!full) {
       __syncthreads();                                          // the last run's map has been read
       if (threadIdx.x < BS) map[threadIdx.x] = -1;
       if (threadIdx.x == BS) earlier = 0;
       __syncthreads();
-      for (int i = threadIdx.x; i < w.num_tokens; i += 256) {
-        const int64_t s = w.slots[i];
-        if (block_of(s) != block) continue;
-        if (i < t) earlier = 1;
-        else atomicMax(&map[s % BS], i);                        // of two tokens for one slot the later one
+      for (int i0 = threadIdx.x; i0 < w.num_tokens; i0 += 256 * kScLook) {
+        int64_t s[kScLook];
+#pragma unroll
+        for (int k = 0; k < kScLook; ++k) s[k] = slot_of(i0 + 256 * k);
+#pragma unroll
+        for (int k = 0; k < kScLook; ++k) {
+          const int i = i0 + 256 * k;
+          if (block_of(s[k]) != block) continue;
+          if (i < t) earlier = 1;
+          else atomicMax(&map[s[k] % BS], i);                   // of two tokens for one slot the later one
+        }
       }
       __syncthreads();
       if (earlier) continue;                                    // that entry's workgroup does the block
-      token.map = map;
     }
-    if (head < w.heads) {
-      if (wave & 1) sc_write_values<act_t, E4M3, BS, DMAX>(w, block, head, token, lane);
-      else sc_write_keys<act_t, E4M3, BS, DMAX>(w, block, head, token, lane);
+    if (head >= w.heads) continue;
+    if (full) {
+      if (wave & 1) sc_write_values<act_t, E4M3, BS, DMAX, true>(w, block, head, nullptr, t, lane);
+      else sc_write_keys<act_t, E4M3, BS, DMAX, true>(w, block, head, nullptr, t, lane);
+    } else {
+      if (wave & 1) sc_write_values<act_t, E4M3, BS, DMAX, false>(w, block, head, map, 0, lane);
+      else sc_write_keys<act_t, E4M3, BS, DMAX, false>(w, block, head, map, 0, lane);
     }
   }
 }
 
-// One wave: K or V of one (block, head) of one sequence.
+// One wave: K or V of one (block, head) of one sequence.  A lane's 16 bytes of a key block are 16 dims of a token, written as they are.
+// Of a value block they are 16 tokens of two dims: lane (c, q) = (lane & 15, lane >> 4) takes dims 8 c + 2 q and the next, and has, in
+// exchange with the three lanes 16 apart, 4 tokens of dims 8 c .. 8 c + 7, a token's 16 bytes each.  Bound by memory, whose writes are
+// hurt by too many of them under way: 5 workgroups of a compute unit (kScReadLds) and stores past the caches.  9 sequences of some 6000
+// tokens, 8 heads of 128, 353 MB: 80 us (8 workgroups 87; 4-byte stores of values 84 / 91; two and four blocks a wave 86 and 91 where one
+// took 84).
+constexpr int kScReadLds = 32 * 1000;                          // bytes that a launch asks for and does not use
+
 template <typename act_t, bool E4M3, int BS, int DMAX>
 __global__ void __launch_bounds__(256) scaled_read_kernel(const ScRead w) {
   using A = ScAct<act_t>;
   using S = typename A::S;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int head = blockIdx.y * 2 + (wave >> 1), seq = blockIdx.z;
+  const int page = blockIdx.x / w.head_pairs, head = (blockIdx.x - page * w.head_pairs) * 2 + (wave >> 1), seq = blockIdx.y;
   const int64_t first = w.starts[seq];
   const int64_t len = min((int64_t)w.lens[seq], (int64_t)w.width * BS);
-  const int at0 = blockIdx.x * BS;
+  const int at0 = page * BS;
   if (head >= w.heads || at0 >= len || first < 0) return;
   // rows behind the end of the output are not written
-  const int count = (int)min((int64_t)min((int64_t)BS, len - at0), w.num_rows - first - at0);
-  const int block = w.tables[(int64_t)seq * w.table_stride + blockIdx.x];
+  const int count = (int)min(min((int64_t)BS, len - at0), w.num_rows - first - at0);
+  const int block = w.tables[(int64_t)seq * w.table_stride + page];
   const bool good = block >= 0 && block < w.num_blocks;        // tokens of blocks that do not exist are zeros
   const int64_t bh = (int64_t)(good ? block : 0) * w.heads + head;
   const int kv = wave & 1;
@@ -276,53 +356,74 @@ __global__ void __launch_bounds__(256) scaled_read_kernel(const ScRead w) {
   const uint8_t* in = w.cache[kv] + bh * w.head_size * BS;
   S* out = reinterpret_cast<S*>(w.x[kv]) + (first + at0) * w.stride[kv] + (int64_t)head * w.head_size;
   if (kv == 0) {
-    constexpr int NU = (BS * DMAX / 16 + 63) / 64;
-    const int chunks = w.head_size >> 4;
+    constexpr int NU = (BS * DMAX / 16 + 63) / 64, STEP = 64 / BS;
+    const int chunks = w.head_size >> 4, t = lane % BS, c0 = lane / BS;
+    sc_u32x4 q[NU];
+#pragma unroll
+    for (int i = 0; i < NU; ++i)
+      q[i] = good && c0 + i * STEP < chunks ? reinterpret_cast<const sc_u32x4*>(in)[lane + 64 * i] : sc_u32x4{0u, 0u, 0u, 0u};
+    if (t >= count) return;
+    S* row = out + t * w.stride[0] + 16 * c0;
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
-      const int u = lane + 64 * i, t = u / chunks, c = u - t * chunks;
-      if (t >= count) continue;
-      const sc_u32x4 q = good ? *reinterpret_cast<const sc_u32x4*>(in + (c * BS + t) * 16) : sc_u32x4{0u, 0u, 0u, 0u};
+      if (c0 + i * STEP >= chunks) continue;
       float o[16];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) ScCode<E4M3>::decode(q[k], o + 4 * k);
-      sc_u32x4* p = reinterpret_cast<sc_u32x4*>(out + t * w.stride[0] + 16 * c);
+      for (int k = 0; k < 4; ++k) ScCode<E4M3>::scaled(q[i][k], scale, o + 4 * k);
+      sc_u32x4* p = reinterpret_cast<sc_u32x4*>(row + 16 * STEP * i);
 #pragma unroll
       for (int k = 0; k < A::kWords / 4; ++k) {
         sc_u32x4 v;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if constexpr (sizeof(S) == 2) v[e] = A::pair(o[8 * k + 2 * e] * scale, o[8 * k + 2 * e + 1] * scale);
-          else v[e] = __float_as_uint(o[4 * k + e] * scale);
+          if constexpr (sizeof(S) == 2) v[e] = A::pair(o[8 * k + 2 * e], o[8 * k + 2 * e + 1]);
+          else v[e] = __float_as_uint(o[4 * k + e]);
         }
-        p[k] = v;
+        __builtin_nontemporal_store(v, p + k);
       }
     }
   } else {
+    constexpr int NP = DMAX / 128, H = BS == 32 ? 2 : 1, RW = BS < 16 ? BS / 4 : 4;
+    const int c0 = lane & 15, q0 = lane >> 4;
+    uint32_t r[NP][H][2][4];
 #pragma unroll
-    for (int i = 0; i < DMAX / 128; ++i) {
-      const int p = lane + 64 * i;
-      if (p >= w.head_size >> 1) continue;
-      const uint32_t* row = reinterpret_cast<const uint32_t*>(in + (int64_t)2 * p * BS);
-      uint32_t q[2][BS / 4];
+    for (int i = 0; i < NP; ++i) {
+      const uint32_t d = 8 * (c0 + 16 * i) + 2 * q0;
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+      for (int h = 0; h < H; ++h)
 #pragma unroll
-        for (int k = 0; k < BS / 4; ++k) q[e][k] = good ? row[e * (BS / 4) + k] : 0u;
+        for (int e = 0; e < 2; ++e)
 #pragma unroll
-      for (int k = 0; k < BS / 4; ++k) {
-        float a[4], b[4];
-        ScCode<E4M3>::decode(q[0][k], a);
-        ScCode<E4M3>::decode(q[1][k], b);
+          for (int k = 0; k < 4; ++k)
+            r[i][h][e][k] = k < RW && good && (int)d < w.head_size ? reinterpret_cast<const uint32_t*>(in + ((d + e) * BS + 16 * h))[k] : 0u;
+    }
+    const uint32_t lane_off = (uint32_t)(4 * q0 * w.stride[1] + 8 * c0) * sizeof(S);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (4 * k + e >= count) continue;
-          S* to = out + (4 * k + e) * w.stride[1] + 2 * p;
-          if constexpr (sizeof(S) == 2) *reinterpret_cast<uint32_t*>(to) = A::pair(a[e] * scale, b[e] * scale);
-          else *reinterpret_cast<sc_u32x2*>(to) = sc_u32x2{__float_as_uint(a[e] * scale), __float_as_uint(b[e] * scale)};
+    for (int i = 0; i < NP; ++i)
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        sc_transpose(r[i][h][0]);
+        sc_transpose(r[i][h][1]);
+        float o[8][4];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ScCode<E4M3>::scaled(r[i][h][e & 1][e >> 1], scale, o[e]);
+        if (8 * (c0 + 16 * i) >= w.head_size) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (16 * h + 4 * q0 + j >= count) continue;
+          char* to = reinterpret_cast<char*>(out + (16 * h + j) * w.stride[1] + 128 * i) + lane_off;
+          if constexpr (sizeof(S) == 2) {
+            const sc_u32x4 v = {A::pair(o[0][j], o[1][j]), A::pair(o[2][j], o[3][j]), A::pair(o[4][j], o[5][j]), A::pair(o[6][j], o[7][j])};
+            __builtin_nontemporal_store(v, reinterpret_cast<sc_u32x4*>(to));
+          } else {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const sc_u32x4 v = {__float_as_uint(o[4 * k][j]), __float_as_uint(o[4 * k + 1][j]), __float_as_uint(o[4 * k + 2][j]), __float_as_uint(o[4 * k + 3][j])};
+              __builtin_nontemporal_store(v, reinterpret_cast<sc_u32x4*>(to) + k);
+            }
+          }
         }
       }
-    }
   }
 }
 
@@ -389,8 +490,12 @@ int sw_reshape_and_cache_scaled(const void* key, const void* value, void* key_ca
   w.num_slots = num_blocks * block_size;
   w.num_tokens = num_tokens, w.heads = num_heads, w.head_size = head_size;
   // a decode step's entries each begin a run, a prompt's only every block_size-th
-  w.window = num_tokens <= 1024 ? 1 : block_size;
-  const dim3 grid((num_tokens + w.window - 1) / w.window, (num_heads + 1) / 2);
+  static_assert(1 + kScWindow + 32 <= 64, "");
+  w.window = num_tokens <= 1024 ? 1 : kScWindow;
+  w.head_pairs = (num_heads + 1) / 2;
+  const int64_t workgroups = ((int64_t)num_tokens + w.window - 1) / w.window * w.head_pairs;
+  SW_CHECK_ARG(workgroups <= INT32_MAX, "reshape_and_cache_scaled: %d tokens of %d heads are too many for a call", num_tokens, num_heads);
+  const dim3 grid((unsigned)workgroups);
   return sc_by_type(act_dtype, cache_dtype, [&](auto a, auto e) {
     return sc_by_size(head_size, block_size, [&](auto bs, auto d) -> int {
       scaled_write_kernel<decltype(a), decltype(e)::value, decltype(bs)::value, decltype(d)::value>
@@ -425,11 +530,14 @@ int sw_gather_cache_scaled(void* key, void* value, const void* key_cache, const 
   w.num_blocks = (int)num_blocks, w.width = max_blocks_per_seq, w.heads = num_heads, w.head_size = head_size;
   const int blocks = std::min((int)(((int64_t)max_seq_len + block_size - 1) / block_size), max_blocks_per_seq);
   if (num_seqs == 0 || blocks == 0 || num_rows == 0) return SW_OK;
-  const dim3 grid(blocks, (num_heads + 1) / 2, num_seqs);
+  w.head_pairs = (num_heads + 1) / 2;
+  SW_CHECK_ARG((int64_t)blocks * w.head_pairs <= INT32_MAX, "gather_cache_scaled: sequences of %d blocks of %d heads are too long for a call",
+               blocks, num_heads);
+  const dim3 grid(blocks * w.head_pairs, num_seqs);
   return sc_by_type(act_dtype, cache_dtype, [&](auto a, auto e) {
     return sc_by_size(head_size, block_size, [&](auto bs, auto d) -> int {
       scaled_read_kernel<decltype(a), decltype(e)::value, decltype(bs)::value, decltype(d)::value>
-          <<<grid, 256, 0, (hipStream_t)stream>>>(w);
+          <<<grid, 256, kScReadLds, (hipStream_t)stream>>>(w);
       SW_CHECK_LAUNCH();
       return SW_OK;
     });

@@ -628,6 +628,9 @@ def reshape_and_cache_scaled(key: torch.Tensor, value: torch.Tensor, key_cache: 
     Infinities go to the largest code, NaN to 0.  Slots outside the cache (negative: padding) are skipped.  A block's
     tokens may stand anywhere in the list, and of several for one slot the last one stays (unless neighbours in the list fill the whole
     block in order: then which one does is not specified)."""
+    status = _native.reshape_and_cache_scaled(key, value, key_cache, value_cache, key_scales, value_scales, slot_mapping, kv_cache_dtype)
+    if status is not None:
+        return _check(status)
     name = "reshape_and_cache_scaled"
     _scaled_rows(name, key, value)
     if slot_mapping.dtype != torch.int64 or slot_mapping.shape != (key.shape[0],) or not slot_mapping.is_contiguous():
@@ -648,6 +651,10 @@ def gather_cache_scaled(key: torch.Tensor, value: torch.Tensor, key_cache: torch
     ``seq_starts[i]`` .. of key and value [rows, KVH, D] (fp16, bf16 or fp32), code * scale rounded once.  ``max_seq_len`` bounds the
     lengths (rounded up to whole blocks, no more is read).  Rows of no sequence stay as they are, rows behind the tensors' end are left out,
     and tokens of blocks that do not exist are zeros.  Sequences must not share rows."""
+    status = _native.gather_cache_scaled(key, value, key_cache, value_cache, key_scales, value_scales, block_tables, seq_starts, seq_lens,
+                                         max_seq_len, kv_cache_dtype)
+    if status is not None:
+        return _check(status)
     name = "gather_cache_scaled"
     _scaled_rows(name, key, value)
     _scaled_table(name, block_tables, seq_starts, seq_lens)
@@ -695,6 +702,11 @@ def paged_attention_scaled(out: torch.Tensor, query: torch.Tensor, key_cache: to
     query of sequence i being the last of its ``context_lens[i]`` tokens.  A sequence of no tokens gives zeros, and so does one whose
     blocks do not exist (table entries outside the cache).  ``num_parts``: workgroups that share a context; None lets the library
     decide by the launch's shape and ``max_context_len``."""
+    if alibi_slopes is None and num_parts is None:
+        status = _native.paged_attention_scaled(out, query, key_cache, value_cache, key_scales, value_scales, num_kv_heads, scale,
+                                                block_tables, context_lens, block_size, max_context_len, kv_cache_dtype)
+        if status is not None:
+            return _check(status)
     name = "paged_attention_scaled"
     if query.dim() == 3 and query.shape[0] != block_tables.shape[0]:
         raise RuntimeError(f"{name}: one row of block_tables for each query")
@@ -724,6 +736,12 @@ def context_attention_scaled(out: torch.Tensor, query: torch.Tensor, key_cache: 
     query and out [rows, H, D] (fp16 or bf16) is the sequence's token ``seq_lens[i] - new_lens[i] + j`` and sees the tokens up to itself,
     with ``sliding_window`` the last that many.  ``max_new_len`` and ``max_context_len`` bound new_lens and seq_lens; new tokens beyond the
     former are not computed.  Rows of no sequence stay as they are; sequences must not share rows."""
+    if alibi_slopes is None and num_parts is None:
+        status = _native.context_attention_scaled(out, query, key_cache, value_cache, key_scales, value_scales, scale, block_tables,
+                                                  seq_starts, new_lens, seq_lens, max_new_len, max_context_len, kv_cache_dtype,
+                                                  sliding_window)
+        if status is not None:
+            return _check(status)
     name = "context_attention_scaled"
     num_kv_heads = value_cache.shape[1] if value_cache.dim() == 4 else 0
     cache, alibi_slopes = _scaled_attention(name, out, query, key_cache, value_cache, key_scales, value_scales, num_kv_heads,
