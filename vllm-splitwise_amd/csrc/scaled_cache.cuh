@@ -24,11 +24,14 @@ template <> struct ScCode<false> {
   __device__ static __forceinline__ uint32_t encode(float a, float b, float c, float d) {
     return byte(a) | (byte(b) << 8) | (byte(c) << 16) | (byte(d) << 24);
   }
-  // the same of finite values that a scale of theirs has brought to +-127: 1.5 x 2^23 + v has v's nearest integer in its low byte
+  // the same of finite values that a scale of theirs has brought to +-127: 1.5 x 2^23 + v has v's nearest integer in its low byte.  (Two
+  // roundings: the product's takes what lies on the middle of two codes but for the reciprocal's rounding back there, and so to the even one.)
   __device__ static __forceinline__ uint32_t encode_fitting(float a, float b, float c, float d, float inverse) {
+#pragma clang fp contract(off)
     constexpr float at = 12582912.f;
-    const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(fmaf(b, inverse, at)), __float_as_uint(fmaf(a, inverse, at)), 0x0c0c0400u);
-    const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(fmaf(d, inverse, at)), __float_as_uint(fmaf(c, inverse, at)), 0x04000c0cu);
+    const float pa = a * inverse, pb = b * inverse, pc = c * inverse, pd = d * inverse;
+    const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(pb + at), __float_as_uint(pa + at), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(pd + at), __float_as_uint(pc + at), 0x04000c0cu);
     return lo | hi;
   }
   __device__ static __forceinline__ uint32_t byte(float x) {

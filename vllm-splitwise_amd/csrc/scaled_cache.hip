@@ -113,7 +113,7 @@ constexpr int kScWindow = 16;        // entries of a workgroup; they, one before
 constexpr int kScLook = 16;          // entries that a thread asks for at a time as it goes through the list
 
 // Bound by vector instructions as much as by memory (an element is 2 bytes in and 1 out), so: a lane's addresses are one number and what
-// the compiler can put into the instructions; magnitudes two at a time; codes of finite values, the rule, in 3 instructions an element; and
+// the compiler can put into the instructions; magnitudes two at a time; codes of finite values, the rule, in 4 instructions an element; and
 // blocks that the call fills look at no single token.
 
 // A lane's pieces are 16 elements of the key of one token, the same for all its pieces: 32 bytes in (64 of fp32), 16 out, where a wave's lie
