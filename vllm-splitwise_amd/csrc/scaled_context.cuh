@@ -7,10 +7,10 @@
 //     v_mfma_f32_32x32x16_f16: S^T = K . Q^T [32 tokens x 32 rows], O^T += V^T . P^T [32 dims x 32 rows].  A row is a lane's column in both;
 //   * the accumulator of S^T is P^T's operand as it stands: lane half h has tokens 8 b + 4 h + j, so values are laid down with the tokens of
 //     a run of 16 in the order 0-3, 8-11, 4-7, 12-15;
-//   * scales come as three numbers for each 8 tokens, made by 8 threads for all: the key scale; log2 of the value scale over the reference
-//     (the largest so far), which goes into the weight's exponent; and its reciprocal, which takes it out of the weights' sum again.
-//     A score costs one product-and-sum, one exp2, one addition, half a maximum and half a packing;
-//   * sums are rescaled only where a row's maximum has grown by more than 2^8 or the reference has.
+//   * scales come as three numbers for each 8 tokens, made by 8 threads for all: the key scale; log2 of the value scale, which goes, less
+//     the reference (the largest's, but for 2^6), into the weight's exponent; and its reciprocal, which takes it out of the weights' sum
+//     again.  A score costs one product-and-sum, one exp2, one addition, half a maximum and half a packing;
+//   * sums are rescaled only where a row's maximum has grown by more than 2^8 or a value scale by more than 2^6.
 #pragma once
 
 #include "scaled_attention.cuh"
@@ -21,7 +21,9 @@ using sc_f32x16 = __attribute__((ext_vector_type(16))) float;
 
 constexpr int kScRows = 32;                                   // of a wave
 constexpr float kScLazy = 8.f;                                // powers of two by which a weight may pass 1
+constexpr float kScHigher = 6.f;                              // and by which a value scale may pass the reference: both fit a half
 constexpr float kScDeep = 40.f;                               // below the reference by more a value scale counts as that much below it
+constexpr float kScLeast = 0x1p-120f;                         // and below this as this (a block of zeros has the scale 0)
 
 constexpr int kScSteps = 8;                                   // dwords of codes of a key's piece and a value's
 
@@ -121,7 +123,6 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
   sc_u32x4 kraw[NP], vraw[NP], keep = {0u, 0u, 0u, 0u};
   float kscale = 0.f, vscale = 0.f;
   bool sgood = false;
-  float reference = -INFINITY;                                // of threads 0 .. SB - 1: log2 of the largest value scale so far
   auto look = [&](int t0) {
 #pragma unroll
     for (int b = 0; b < PB; ++b) runblock[b] = entry(t0 + 16 * run + 8 * b);
@@ -182,27 +183,20 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
     }
   };
   auto lay = [&](int buf) { static_for<kScSteps * NP>([&](auto K) { lay_step(K, buf); }); };
-  auto lay_scales = [&](int t0, int buf) {
+  // eight tokens' key scale, log2 of the value scale, its reciprocal; and which eights do not exist
+  auto lay_scales = [&](int buf) {
     if (tid < SB) {
       float* f = reinterpret_cast<float*>(smem + buf * BUFFER + KT * KSTRIDE + sc_padded(HEAD) * VSTRIDE);
-      const float there = t0 + 8 * tid < s.len && vscale > 0.f ? __builtin_amdgcn_logf(vscale) : -INFINITY;
-      float top = there;
-#pragma unroll
-      for (int m = 1; m < SB; m <<= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-      reference = fmaxf(reference, top);
-      const float from = sc_base(reference), below = fmaxf(there - from, -kScDeep);
+      const float v = fmaxf(vscale, kScLeast);
       f[tid] = kscale;
-      f[8 + tid] = vscale != vscale ? vscale : below;         // (a NaN of a scale reaches the rows that see its block)
-      f[16 + tid] = __builtin_amdgcn_exp2f(-below);
+      f[8 + tid] = vscale != vscale ? vscale : __builtin_amdgcn_logf(v);      // (a NaN of a scale reaches the rows that see its block)
+      f[16 + tid] = __builtin_amdgcn_rcpf(v);
       const uint64_t missing = __ballot(!sgood);
-      if (tid == 0) {
-        f[24] = from;
-        reinterpret_cast<uint32_t*>(f)[25] = (uint32_t)(missing & ((1u << SB) - 1u));
-      }
+      if (tid == 0) reinterpret_cast<uint32_t*>(f)[24] = (uint32_t)(missing & ((1u << SB) - 1u));
     }
   };
 
-  float m_run = -INFINITY, l_run = 0.f, ref_run = 0.f;
+  float m_run = -INFINITY, l_run = 0.f, ref_run = -INFINITY;   // (the reference: of the wave, whose rows' sums are in units of 2 to it)
   sc_f32x16 o[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b)
@@ -216,7 +210,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
     fetch(first);
     look(first + KT);
     lay(0);
-    lay_scales(first, 0);
+    lay_scales(0);
     fetch(first + KT);
     look(first + 2 * KT);
     __syncthreads();
@@ -224,7 +218,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
   int buf = 0;
   for (int st = 0; st < stages; ++st, buf ^= 1) {
     const int t0 = first + st * KT;
-    lay_scales(t0 + KT, buf ^ 1);
+    lay_scales(buf ^ 1);
     if (!(active && t0 <= wave_high && t0 + KT > wave_from)) {
       lay(buf ^ 1);
       fetch(t0 + 2 * KT);
@@ -239,9 +233,10 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
       for (int u = 0; u < NT; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[u][i] = 0.f;
-      float fs[SB];
+      float fs[SB], log_v[SB];
 #pragma unroll
-      for (int b = 0; b < SB; ++b) fs[b] = f[b] * row_scale;
+      for (int b = 0; b < SB; ++b) fs[b] = f[b] * row_scale, log_v[b] = f[8 + b];
+      const uint32_t missing = __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint32_t*>(f)[24]);
       auto top_of = [&](int b) {
         const int u = b >> 2, i = (b & 3) * 4;
         return fmaxf(fmaxf(x[u][i], x[u][i + 1]), fmaxf(x[u][i + 2], x[u][i + 3])) * fs[b];
@@ -271,8 +266,6 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
       look(t0 + 3 * KT);
 
       // scores in powers of two: x fs, where no row has anything to hide or to add
-      const uint32_t missing = __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint32_t*>(f)[25]);
-      const float ref = f[24];
       if (t0 + KT > wave_low + 1 || t0 < none_hidden || missing || a.slopes) {
 #pragma unroll
         for (int u = 0; u < NT; ++u)
@@ -293,19 +286,32 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
 #pragma unroll
       for (int b = SB - 4; b < SB; ++b) top = fmaxf(top, top_of(b));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      if (__any(top > m_run + kScLazy) || ref != ref_run) {
-        const float m_new = fmaxf(m_run, top);
+      // (all lanes have the same scales)
+      float most_v = log_v[0], least_v = log_v[0];
+#pragma unroll
+      for (int b = 1; b < SB; ++b) most_v = fmaxf(most_v, log_v[b]), least_v = fminf(least_v, log_v[b]);
+      if (__any(top > m_run + kScLazy || most_v > ref_run + kScHigher)) {
+        const float m_new = fmaxf(m_run, top), ref_new = most_v > ref_run + kScHigher ? most_v : ref_run;
         const float alpha = __builtin_amdgcn_exp2f(m_run - sc_base(m_new));
         m_run = m_new;
         l_run *= alpha;
-        const float shrink = alpha > 0.f ? alpha * __builtin_amdgcn_exp2f(ref_run - ref) : 0.f;   // (the first reference may be any)
-        ref_run = ref;
+        const float shrink = ref_run == -INFINITY ? 0.f : alpha * __builtin_amdgcn_exp2f(ref_run - ref_new);
+        ref_run = ref_new;
 #pragma unroll
         for (int b = 0; b < DB; ++b)
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[b][i] *= shrink;
       }
-      const float base = sc_base(m_run);
+      const float unit = __builtin_amdgcn_exp2f(ref_run);
+      float undo[SB];
+#pragma unroll
+      for (int b = 0; b < SB; ++b) undo[b] = f[16 + b] * unit;
+      if (__any(least_v < ref_run - kScDeep)) {
+#pragma unroll
+        for (int b = 0; b < SB; ++b)
+          if (log_v[b] < ref_run - kScDeep) log_v[b] = ref_run - kScDeep, undo[b] = __builtin_amdgcn_exp2f(kScDeep);
+      }
+      const float base = sc_base(m_run) + ref_run;
       // Weights of a run of 16 tokens, a few between each two products of the run before.
       const char* vp = v_img + col * VSTRIDE + half * 16;
       constexpr int RN = 2 * NT;
@@ -313,13 +319,13 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
       sc_u32x4 pf;
       auto weigh = [&](auto N_, auto E) {
         constexpr int n = decltype(N_)::value, e = decltype(E)::value, b = 2 * n + e / 4;
-        if constexpr (e % 4 == 0) shift = f[8 + b] - base;
+        if constexpr (e % 4 == 0) shift = log_v[b] - base;
         p[e] = __builtin_amdgcn_exp2f(fmaf(x[b >> 2][(b & 3) * 4 + e % 4], fs[b], shift));
       };
       auto pack = [&](auto N_) {
         constexpr int n = decltype(N_)::value;
-        l_run = fmaf((p[0] + p[1]) + (p[2] + p[3]), f[16 + 2 * n], l_run);
-        l_run = fmaf((p[4] + p[5]) + (p[6] + p[7]), f[17 + 2 * n], l_run);
+        l_run = fmaf((p[0] + p[1]) + (p[2] + p[3]), undo[2 * n], l_run);
+        l_run = fmaf((p[4] + p[5]) + (p[6] + p[7]), undo[2 * n + 1], l_run);
 #pragma unroll
         for (int w = 0; w < 4; ++w) pf[w] = sc_pack_f16(p[2 * w], p[2 * w + 1]);
       };
@@ -348,7 +354,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
 
   l_run += __shfl_xor(l_run, 32, 64);
   if (!real) return;
-  const float unit = __builtin_amdgcn_exp2f(ref_run);
+  const float unit = ref_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref_run);
   const float inv = a.partial ? unit : l_run > 0.f ? unit / l_run : l_run != l_run ? l_run : 0.f;   // a row that sees nothing gives zeros
   float* to = nullptr;
   uint16_t* out = nullptr;
