@@ -177,3 +177,29 @@ def test_oracle_codes_go_both_ways(kind):
     assert torch.equal(oracle.cache_of(oracle.codes_of(raw, kind), kind, True), raw)
     raw = raw.view(3, 2, 64, 8)
     assert torch.equal(oracle.cache_of(oracle.codes_of(raw, kind), kind, False), raw)
+
+
+# ------------------------------------------------------------------------------------------- engine options
+def test_engine_options_that_a_cache_with_scales_excludes():
+    from splitwise_amd.config import CacheConfig
+    from splitwise_amd.engine.arg_utils import EngineArgs
+    for kind in ("int8", "fp8_e4m3"):
+        assert CacheConfig(16, 0.9, 0, kind, enable_prefix_caching=True).cache_dtype == kind
+        with pytest.raises(NotImplementedError, match="sliding window"):
+            CacheConfig(16, 0.9, 0, kind, sliding_window=64)
+        for more in (dict(sep_prompt_token=True), dict(overlap_prompt_decode=True, pipeline_steps=True)):
+            with pytest.raises(NotImplementedError, match="scales"):
+                EngineArgs(model="llama-tiny", kv_cache_dtype=kind, **more).create_engine_configs()
+    with pytest.raises(NotImplementedError, match="prefix caching"):
+        CacheConfig(16, 0.9, 0, "fp8_e5m2", enable_prefix_caching=True)
+    with pytest.raises(ValueError, match="Unknown kv cache dtype"):
+        CacheConfig(16, 0.9, 0, "int4")
+
+
+def test_scales_count_in_a_block():
+    import types
+    from splitwise_amd.worker.cache_engine import CacheEngine
+    model = types.SimpleNamespace(dtype=torch.bfloat16, get_head_size=lambda: 64, get_num_layers=lambda p: 3, get_num_kv_heads=lambda p: 2)
+    size = lambda kind: CacheEngine.get_cache_block_size(16, kind, model, None)  # noqa: E731
+    assert size("auto") == 3 * 2 * 16 * 2 * 64 * 2 and size("fp8_e5m2") == size("auto") // 2
+    assert size("int8") == size("fp8_e4m3") == size("fp8_e5m2") + 3 * 2 * 2 * 4

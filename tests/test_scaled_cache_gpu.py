@@ -489,7 +489,7 @@ def test_captured_and_replayed(kind):
     for t, k in zip(c.device, keep):
         t.copy_(k)
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
+    with torch.inference_mode(), torch.cuda.graph(graph):      # (as the workers capture: one process takes one kind)
         step(c, out, read)
     for i in range(4):
         g = torch.Generator().manual_seed(i)

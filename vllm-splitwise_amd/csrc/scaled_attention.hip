@@ -123,7 +123,7 @@ ScPlan sc_plan(int num_seqs, int max_new_len, int num_heads, int num_kv_heads, i
     // kv heads 1 17.2, 4 12.2, 8 10.9, 32 11.9; 4 x 6001 1 60.9, 4 25.5, 8 18.1, 16 23.1; 32 heads, 1 x 501 1 8.6, 2 10.6; 4 and 8 waves:
     // 64 x 1000 of 8 heads 38.9 / 41.5, 32 x 8192 143 / 117, 128 x 4096 220 / 212).
     const int64_t w = workgroups(16);
-    p.waves = head_size <= 128 && w <= (max_context_len >= 4096 ? 1024 : 256) ? 8 : 4;
+    p.waves = head_size <= 128 && w <= (max_context_len >= 4096 && rows <= 16 ? 1024 : 256) ? 8 : 4;
     p.parts = (int)std::min<int64_t>(max_context_len < 1024 ? 1 : ((int64_t)max_context_len + 255) / 256, 256 / w);
   } else {
     // 256 rows where there are enough of them: half the widening a row (us, 128 / 256 rows: 2041 tokens of 8 heads behind 14003 1127 /

@@ -345,8 +345,13 @@ class ModelConfig:
         return None
 
 
+# 8-bit codes with one fp32 scale for each (block, kv head)
+SCALED_CACHE_DTYPES = ("int8", "fp8_e4m3")
+
+
 class CacheConfig:
-    """vllm/config.py:334-388.  fp8_e5m2 is allowed on ROCm here (the reference refuses it)."""
+    """vllm/config.py:334-388.  fp8_e5m2 is allowed on ROCm here (the reference refuses it).  "int8" and "fp8_e4m3", which the
+    reference does not have, keep 8-bit codes with a scale for each (block, kv head) (``SCALED_CACHE_DTYPES``)."""
 
     def __init__(self, block_size: int, gpu_memory_utilization: float, swap_space: float,
                  cache_dtype: str = "auto", sliding_window: Optional[int] = None,
@@ -359,11 +364,14 @@ class CacheConfig:
         self.enable_prefix_caching = enable_prefix_caching
         if gpu_memory_utilization > 1.0:
             raise ValueError(f"GPU memory utilization must be less than 1.0. Got {gpu_memory_utilization}.")
-        if cache_dtype not in ("auto", "fp8_e5m2"):
+        if cache_dtype not in ("auto", "fp8_e5m2") + SCALED_CACHE_DTYPES:
             raise ValueError(f"Unknown kv cache dtype: {cache_dtype}")
-        if enable_prefix_caching and cache_dtype != "auto":
-            # the prefix-aware prompt kernel reads the cached context in the activation dtype
-            raise NotImplementedError("prefix caching needs kv_cache_dtype 'auto'")
+        if enable_prefix_caching and cache_dtype == "fp8_e5m2":
+            # the prefix-aware prompt kernels read the cached context in the activation dtype or with its scales
+            raise NotImplementedError("prefix caching needs kv_cache_dtype 'auto', 'int8' or 'fp8_e4m3'")
+        if cache_dtype in SCALED_CACHE_DTYPES and sliding_window is not None:
+            # a window's blocks are used again in place, and a block's first token starts its scale over
+            raise NotImplementedError(f"models with a sliding window need kv_cache_dtype 'auto' or 'fp8_e5m2', not {cache_dtype!r}")
         self.num_gpu_blocks: Optional[int] = None
         self.num_cpu_blocks: Optional[int] = None
 

@@ -5,7 +5,7 @@ import dataclasses
 from dataclasses import dataclass
 from typing import Optional, Tuple
 
-from ..config import CacheConfig, DeviceConfig, ModelConfig, ParallelConfig, SchedulerConfig
+from ..config import SCALED_CACHE_DTYPES, CacheConfig, DeviceConfig, ModelConfig, ParallelConfig, SchedulerConfig
 
 
 @dataclass
@@ -62,6 +62,9 @@ class EngineArgs:
         cache_config = CacheConfig(self.block_size, self.gpu_memory_utilization, self.swap_space,
                                    self.kv_cache_dtype, model_config.get_sliding_window(),
                                    self.enable_prefix_caching)
+        if self.kv_cache_dtype in SCALED_CACHE_DTYPES and (self.sep_prompt_token or self.overlap_prompt_decode):
+            raise NotImplementedError(f"kv_cache_dtype {self.kv_cache_dtype!r} keeps scales beside the cache, which the transport between "
+                                      "prompt and token pools does not carry: it excludes sep_prompt_token and overlap_prompt_decode")
         if self.overlap_prompt_decode:
             # the engine runs its split loop (a prompt side and a token side that run free of each other) over ONE
             # worker: executor/overlap_executor.py

@@ -18,6 +18,7 @@ import torch
 import torch.nn as nn
 
 from ... import _C
+from ...config import SCALED_CACHE_DTYPES
 from ..input_metadata import InputMetadata
 
 _PARTITION_SIZE = 512          # must match the partition size of sw_paged_attention_v2
@@ -34,6 +35,10 @@ class PagedAttentionImpl:
     @staticmethod
     def reshape_and_cache(key, value, key_cache, value_cache, input_metadata: InputMetadata) -> None:
         slots = input_metadata.slot_mapping
+        if input_metadata.kv_cache_dtype in SCALED_CACHE_DTYPES:
+            _C.cache_ops.reshape_and_cache_scaled(key, value, key_cache, value_cache, *key_cache.scales, slots.flatten(),
+                                                  input_metadata.kv_cache_dtype)
+            return
         _C.cache_ops.reshape_and_cache(key, value, key_cache, value_cache, slots if slots.dim() == 1 else slots.flatten(),
                                        input_metadata.kv_cache_dtype)
 
@@ -144,12 +149,20 @@ class PagedAttentionImpl:
 
     @staticmethod
     def forward_prefix(query, key, value, key_cache, value_cache, input_metadata: InputMetadata,
-                       alibi_slopes=None):
+                       alibi_slopes=None, scale=None):
         """Prompt attention of new tokens over a prefix that is already in the cache
         (ops/paged_attn.py:113-138): query / key / value [T, heads, head_size] of the new tokens;
         the metadata carries the block tables, the first row of each sequence (start_loc), the
-        total lengths (prompt_lens) and the cached lengths (context_lens)."""
+        total lengths (prompt_lens) and the cached lengths (context_lens).  A cache with scales is read for the new
+        tokens too, which have been written there.  ``scale``: head_size^-1/2 if None; a 16-bit cache's kernel knows no other."""
         output = torch.empty_like(query)
+        if input_metadata.kv_cache_dtype in SCALED_CACHE_DTYPES:
+            tables, lens = input_metadata.block_tables, input_metadata.prompt_lens
+            _C.ops.context_attention_scaled(output, query, key_cache, value_cache, *key_cache.scales,
+                                            query.shape[2] ** -0.5 if scale is None else scale, tables, input_metadata.start_loc,
+                                            lens - input_metadata.context_lens, lens, input_metadata.max_seq_len,
+                                            tables.shape[1] * value_cache.shape[3], alibi_slopes, input_metadata.kv_cache_dtype)
+            return output
         _C.ops.context_attention_fwd(query, key, value, output, key_cache, value_cache, input_metadata.block_tables,
                                      input_metadata.start_loc, input_metadata.prompt_lens,
                                      input_metadata.context_lens, input_metadata.max_seq_len, alibi_slopes)
@@ -163,6 +176,13 @@ class PagedAttentionImpl:
         block_size = value_cache.shape[3]
         num_seqs, num_heads, head_size = query.shape
         max_ctx = input_metadata.max_context_len
+        if input_metadata.kv_cache_dtype in SCALED_CACHE_DTYPES:
+            if key is not None:
+                PagedAttentionImpl.reshape_and_cache(key, value, key_cache, value_cache, input_metadata)
+            _C.ops.paged_attention_scaled(output, query, key_cache, value_cache, *key_cache.scales, num_kv_heads, scale,
+                                          input_metadata.block_tables, input_metadata.context_lens, block_size, max_ctx, alibi_slopes,
+                                          input_metadata.kv_cache_dtype)
+            return output
         width = PagedAttentionImpl.query_group_width(num_heads, num_kv_heads, head_size, block_size, query.dtype,
                                                      input_metadata.kv_cache_dtype)
         forced = getattr(input_metadata, "decode_kernel", None)
@@ -237,8 +257,9 @@ class Attention(nn.Module):
         launch, any other step applies ``rotary`` first and goes on as the reference does."""
         out_shape = query.shape
         fused_cache_write = False
+        scaled = input_metadata.kv_cache_dtype in SCALED_CACHE_DTYPES        # its write and its attentions are calls of their own
         if rotary is not None:
-            if (not input_metadata.is_prompt and key_cache is not None and value_cache is not None
+            if (not scaled and not input_metadata.is_prompt and key_cache is not None and value_cache is not None
                     and rotary.fusable_with_cache_write(query.dtype)):
                 _C.ops.rotary_embedding_and_cache(positions.flatten(), query, key, value, key_cache, value_cache,
                                                   input_metadata.slot_mapping.flatten(), self.head_size,
@@ -258,7 +279,7 @@ class Attention(nn.Module):
 
         tables = input_metadata.block_tables
         writes_cache = key_cache is not None and value_cache is not None and not fused_cache_write
-        if (writes_cache and input_metadata.is_prompt and (tables is None or tables.numel() == 0)
+        if (writes_cache and not scaled and input_metadata.is_prompt and (tables is None or tables.numel() == 0)
                 and not (input_metadata.blocks_to_nw and self.kvcache_comm_manager is not None)
                 and PagedAttentionImpl.writes_beside_prompt(query.shape[0], input_metadata.prompt_lens.numel(),
                                                             input_metadata.max_seq_len, self.num_heads, self.num_kv_heads,
@@ -295,7 +316,7 @@ class Attention(nn.Module):
                 # some prompt of the step continues a prefix that is in the cache already: the new tokens
                 # attend to the paged context and to each other (backends/xformers.py:166-177)
                 output = PagedAttentionImpl.forward_prefix(query, key, value, key_cache, value_cache, input_metadata,
-                                                           self.alibi_slopes)
+                                                           self.alibi_slopes, self.scale)
             else:
                 output = torch.empty_like(query)
                 _C.ops.prefill_attention(output, query, key, value, input_metadata.start_loc,

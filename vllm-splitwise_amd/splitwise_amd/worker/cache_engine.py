@@ -5,13 +5,16 @@ Same layout and accounting as vllm/worker/cache_engine.py:15-178: per layer a ke
 value cache [num_blocks, kv_heads, head_size, block_size]; pinned host mirrors for swapping;
 swap / copy run on a side stream with one event per layer.  This layout is also the wire
 format of the KV push between the prompt and token pools, so it is kept bit for bit.
+
+Caches of 8-bit codes with a scale for each (block, kv head) (``cache_dtype`` "int8" / "fp8_e4m3") have the same layout; their
+scales, fp32 [num_blocks, kv_heads] for K and for V, are the key tensor's attribute ``scales`` and go along with every swap and copy.
 """
 from typing import Dict, List, Optional, Tuple
 
 import torch
 
 from .. import _C
-from ..config import CacheConfig, ModelConfig, ParallelConfig
+from ..config import SCALED_CACHE_DTYPES, CacheConfig, ModelConfig, ParallelConfig
 from ..utils import STR_DTYPE_TO_TORCH_DTYPE
 
 KVCache = Tuple[torch.Tensor, torch.Tensor]
@@ -20,7 +23,7 @@ KVCache = Tuple[torch.Tensor, torch.Tensor]
 def _cache_torch_dtype(cache_dtype: str, model_dtype: torch.dtype) -> torch.dtype:
     if cache_dtype == "auto":
         return model_dtype
-    if cache_dtype == "fp8_e5m2":
+    if cache_dtype == "fp8_e5m2" or cache_dtype in SCALED_CACHE_DTYPES:
         return torch.uint8
     return STR_DTYPE_TO_TORCH_DTYPE[cache_dtype]
 
@@ -42,6 +45,13 @@ class CacheEngine:
         self.exported_to_peer = bool(getattr(parallel_config, "sep_prompt_token", False))
         self.gpu_cache = self._allocate_gpu_slab(self.num_gpu_blocks, device)
         self.cpu_cache = self._allocate(self.num_cpu_blocks, torch.device("cpu"), pinned=device.type == "cuda")
+        self.gpu_scales = self.cpu_scales = None
+        if cache_config.cache_dtype in SCALED_CACHE_DTYPES:
+            if self.exported_to_peer:
+                raise NotImplementedError("a cache with scales is not exported to a paired worker")
+            # [layer, K and V, block, kv head]
+            self.gpu_scales = self._attach_scales(self.gpu_cache, self.num_gpu_blocks, device, False)
+            self.cpu_scales = self._attach_scales(self.cpu_cache, self.num_cpu_blocks, torch.device("cpu"), device.type == "cuda")
         self.cache_stream = torch.cuda.Stream(device) if device.type == "cuda" else None
         self.events = ([torch.cuda.Event() for _ in range(self.num_layers)] if device.type == "cuda" else [])
 
@@ -91,6 +101,12 @@ class CacheEngine:
             cache.append((k, v))
         return cache
 
+    def _attach_scales(self, cache: List[KVCache], num_blocks: int, device: torch.device, pinned: bool) -> torch.Tensor:
+        scales = torch.zeros((self.num_layers, 2, num_blocks, self.num_heads), dtype=torch.float32, device=device, pin_memory=pinned)
+        for (k, _), pair in zip(cache, scales):
+            k.scales = (pair[0], pair[1])
+        return scales
+
     def _swap(self, src: List[KVCache], dst: List[KVCache], src_to_dst: Dict[int, int]) -> None:
         # the blocks may still be written by kernels queued on the compute stream
         self.cache_stream.wait_stream(torch.cuda.current_stream(self.device))
@@ -98,6 +114,9 @@ class CacheEngine:
             for layer in range(self.num_layers):
                 _C.cache_ops.swap_blocks(src[layer][0], dst[layer][0], src_to_dst)
                 _C.cache_ops.swap_blocks(src[layer][1], dst[layer][1], src_to_dst)
+                if self.gpu_scales is not None:
+                    for a, b in zip(src[layer][0].scales, dst[layer][0].scales):
+                        _C.cache_ops.swap_blocks(a, b, src_to_dst)
                 self.events[layer].record(stream=self.cache_stream)
 
     def swap_in(self, src_to_dst: Dict[int, int]) -> None:
@@ -109,6 +128,9 @@ class CacheEngine:
     def copy(self, src_to_dsts: Dict[int, List[int]]) -> None:
         # one launch for all layers; runs on the compute stream, so it is ordered before the step
         _C.cache_ops.copy_blocks([k for k, _ in self.gpu_cache], [v for _, v in self.gpu_cache], src_to_dsts)
+        if self.gpu_scales is not None and src_to_dsts:
+            pairs = torch.tensor([(src, dst) for src, dsts in src_to_dsts.items() for dst in dsts]).to(self.gpu_scales.device)
+            self.gpu_scales[:, :, pairs[:, 1]] = self.gpu_scales[:, :, pairs[:, 0]]
 
     @staticmethod
     def get_cache_block_size(block_size: int, cache_dtype: str, model_config: ModelConfig,
@@ -119,7 +141,8 @@ class CacheEngine:
         num_layers = model_config.get_num_layers(parallel_config)
         per_tensor = block_size * num_heads * head_size
         dtype = _cache_torch_dtype(cache_dtype, model_config.dtype)
-        return torch.tensor([], dtype=dtype).element_size() * num_layers * 2 * per_tensor
+        scales = 4 * num_heads if cache_dtype in SCALED_CACHE_DTYPES else 0
+        return num_layers * 2 * (torch.tensor([], dtype=dtype).element_size() * per_tensor + scales)
 
 
 class LayeredCacheEngine:

@@ -23,7 +23,7 @@ from typing import Dict, List, Optional, Tuple
 import numpy as np
 import torch
 
-from ..config import DeviceConfig, ModelConfig, ParallelConfig, SchedulerConfig
+from ..config import SCALED_CACHE_DTYPES, DeviceConfig, ModelConfig, ParallelConfig, SchedulerConfig
 from ..model_executor.input_metadata import InputMetadata, RaggedBatch
 from ..model_executor.layers.sampler import FollowerSamples, PendingSamples, SamplingMetadata
 from ..model_executor.model_loader import get_model
@@ -97,7 +97,8 @@ class ModelRunner:
     def _prompt_rows(self, metas: List[SequenceGroupMetadata]):
         """Per prompt: (new tokens, their positions, their slots, tokens already cached, blocks of those).
         Leading blocks that the block manager reports as computed are skipped: only the rest of the prompt
-        is run, against the cached context (model_runner.py:153-168; prefix caching)."""
+        is run, against the cached context (model_runner.py:153-168; prefix caching).  A cache with scales is read
+        for the new tokens too: there the blocks are the prompt's, all of them."""
         rows = []
         for meta in metas:
             assert meta.is_prompt
@@ -118,14 +119,16 @@ class ModelRunner:
                 # with a sliding window only the last `window` tokens are kept (model_runner.py:195-209)
                 start = 0 if self.sliding_window is None else max(0, n - self.sliding_window)
                 slots = [_PAD_SLOT_ID if i < start else table[i // bs] * bs + i % bs for i in range(computed, n)]
+                if self.kv_cache_dtype in SCALED_CACHE_DTYPES:
+                    prefix = list(table)
             rows.append((tokens[computed:], list(range(computed, n)), slots, computed, prefix))
         return rows
 
     def _prefix_tensors(self, rows):
-        """(cached lengths, block tables of the cached prefixes) as the prompt kernels take them; the table
+        """(cached lengths, block tables of ``_prompt_rows``) as the prompt kernels take them; the table
         has no columns when no prompt of the step has a cached prefix (model_runner.py:236-249)."""
         context_lens = self._to_device(np.asarray([r[3] for r in rows], dtype=np.int32), torch.int32)
-        width = max(len(r[4]) for r in rows)
+        width = max(len(r[4]) for r in rows) if any(r[3] for r in rows) else 0
         if width == 0:
             return context_lens, torch.empty((len(rows), 0), dtype=torch.int32, device=self.device)
         return context_lens, self._to_device(_pad_2d([r[4] for r in rows], width, 0, np.int32), torch.int32)
@@ -423,7 +426,9 @@ class ModelRunner:
         return FollowerSamples(sampling_md.seq_groups, ids)
 
     def _decode_rule(self, num_seqs: int, max_ctx: int, mean_ctx: Optional[float]) -> bool:
-        """PagedAttentionImpl.use_v1 for this model's attention geometry."""
+        """PagedAttentionImpl.use_v1 for this model's attention geometry (a cache with scales has one form of the kernel)."""
+        if self.kv_cache_dtype in SCALED_CACHE_DTYPES:
+            return True
         from ..model_executor.layers.attention import PagedAttentionImpl
         tp = self.parallel_config.tensor_parallel_size
         heads = self.model_config.hf_config["num_attention_heads"] // tp
