@@ -87,7 +87,7 @@ def parse_args():
                     help="wait for a step's tokens before scheduling the next step (the reference's loop)")
     ap.add_argument("--quantization", default=None, choices=[None, "gptq", "awq"],
                     help="int4 weights (fp16 activations); the default workload is unquantised bf16")
-    ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8_e5m2", "int8", "fp8_e4m3"])
+    ap.add_argument("--kv-cache-dtype", default="auto", choices=["auto", "fp8_e5m2"])
     ap.add_argument("--dtype", default=None, help="activation dtype (default bf16, fp16 with --quantization)")
     ap.add_argument("--enforce-eager", action="store_true")
     ap.add_argument("--overlap-prompt-decode", action="store_true",

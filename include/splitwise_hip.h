@@ -434,7 +434,7 @@ int sw_context_attention_split(void* out, const void* query, const void* key, co
  * rescaled.  A token for a block's first slot starts the block over: what it held, scales too, goes, and its other slots are zeros
  * unless the call writes them.  Slots outside 0 .. num_blocks * block_size - 1 are padding.  Tokens of one block may stand anywhere
  * in the list.  Of several tokens for one slot the last one stays, unless one run of neighbours in the list fills the whole block
- * in order: then which one does is not specified. */
+ * in order: then the block's codes and scales may be either's, or some of each. */
 int sw_reshape_and_cache_scaled(const void* key, const void* value, void* key_cache, void* value_cache,
                                 float* key_scales, float* value_scales, const int64_t* slot_mapping, int num_tokens,
                                 int num_heads, int head_size, int block_size, int64_t num_blocks, int64_t key_stride,
@@ -442,7 +442,8 @@ int sw_reshape_and_cache_scaled(const void* key, const void* value, void* key_ca
 
 /* Reads seq_lens[i] tokens of block_tables row i back into rows seq_starts[i] .. of key and value ([num_rows, num_heads,
  * head_size], SW_F32 / SW_F16 / SW_BF16, rows on 16 bytes): code * scale, rounded once.  Tokens from max_seq_len (rounded up to whole
- * blocks) or from max_blocks_per_seq blocks on are not read, rows from num_rows on and those of no sequence not written. */
+ * blocks) or from max_blocks_per_seq blocks on are not read, rows from num_rows on and those of no sequence not written.
+ * value_stride below 2^28 bytes. */
 int sw_gather_cache_scaled(void* key, void* value, const void* key_cache, const void* value_cache,
                            const float* key_scales, const float* value_scales, const int32_t* block_tables,
                            const int32_t* seq_starts, const int32_t* seq_lens, int num_seqs, int max_seq_len,

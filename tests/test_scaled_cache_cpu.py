@@ -150,6 +150,16 @@ def test_entry_points_refuse_before_a_launch(name, changed, why):
     assert status == -1 and why in message, message
 
 
+@pytest.mark.parametrize("name,changed,why", [
+    ("sw_reshape_and_cache_scaled", dict(num_tokens=(1 << 31) - 1, num_heads=256), "too many"),
+    ("sw_gather_cache_scaled", dict(max_seq_len=(1 << 31) - 1, max_blocks_per_seq=1 << 27, num_heads=2), "too long"),
+    ("sw_gather_cache_scaled", dict(value_stride=1 << 26), "2^28 bytes"),
+    ("sw_context_attention_scaled", dict(max_new_len=1 << 24), "new tokens")])
+def test_launches_that_no_grid_holds_are_refused(name, changed, why):
+    status, message = entry_point(name, **changed)
+    assert status == -1 and why in message, message
+
+
 @pytest.mark.parametrize("name,changed", [
     ("sw_paged_attention_scaled", dict(num_seqs=0)), ("sw_context_attention_scaled", dict(num_rows=0)),
     ("sw_context_attention_scaled", dict(max_new_len=0)), ("sw_reshape_and_cache_scaled", dict(num_tokens=0)),

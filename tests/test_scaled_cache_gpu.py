@@ -589,3 +589,148 @@ def test_native_calls_do_the_same(kind, monkeypatch):
         with pytest.raises(RuntimeError, match="heads must be contiguous"):
             _C.ops.paged_attention_scaled(one, query[:2].transpose(1, 2), *c.device, 2, 0.1, tables, i32[2], 16, 700, None, kind)
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+# ------------------------------------------------------------------------- large, wide and repeated calls
+def context(c, query, tables, starts, new, lens, scale, parts=None, out=None, window=None):
+    out = torch.full_like(query, 7.0) if out is None else out
+    _C.ops.context_attention_scaled(out, query, *c.device, scale, tables.to(DEV),
+                                    *(torch.tensor(x, dtype=torch.int32, device=DEV) for x in (starts, new, lens)), max(new), max(lens),
+                                    None, c.kind, sliding_window=window, num_parts=parts)
+    return out
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_cache_past_4_gib(kind):
+    """Blocks on either side of 2^31 and 2^32 bytes and at the cache's end do as the same blocks of a small cache."""
+    heads, size, block, total = 8, 128, 16, 266000             # 16 KiB a block: 4.06 GiB of keys and as much of values
+    far = [0, 131071, 131072, 262143, 262144, 265998, 265999]
+    lens = [40, 37]
+    small = Cache(7, heads, size, block, kind)
+    large = Cache(7, heads, size, block, kind)
+    large.key, large.value = (torch.empty(total, *t.shape[1:], dtype=torch.uint8, device=DEV) for t in (small.key, small.value))
+    large.ks, large.vs = (torch.zeros(total, heads, device=DEV) for _ in range(2))
+    tables = torch.tensor([[6, 1, 3], [4, 2, 5]], dtype=torch.int32)
+    wide = torch.full((2, 5), 1 << 30, dtype=torch.int32)      # rows of a wider table
+    wide[:, 1:4] = torch.tensor(far, dtype=torch.int32)[tables.long()]
+    g = torch.Generator().manual_seed(2)
+    key, value = (torch.randn(sum(lens), heads, size, generator=g).to(torch.bfloat16).to(DEV) for _ in range(2))
+    queries = random_query(sum(lens), 2 * heads, size, torch.bfloat16)
+    results = []
+    for c, t in ((small, tables), (large, wide[:, 1:4])):
+        _C.cache_ops.reshape_and_cache_scaled(key, value, *c.device, slots_of(t, block, [0, 0], lens).to(DEV), kind)
+        rows = [torch.zeros(77, heads, size, dtype=torch.float16, device=DEV) for _ in range(2)]
+        table = torch.nn.functional.pad(t, (1, 1), value=1 << 30).to(DEV)[:, 1:4]
+        i32 = [torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([0, 40], lens)]
+        _C.cache_ops.gather_cache_scaled(*rows, *c.device, table, *i32, 40, kind)
+        outs = []
+        for parts in (1, 2):
+            outs.append(torch.empty_like(queries[:2]))
+            _C.ops.paged_attention_scaled(outs[-1], queries[:2], *c.device, heads, 0.09, table, i32[1], block, 40, None, kind, num_parts=parts)
+            outs.append(torch.empty_like(queries))
+            _C.ops.context_attention_scaled(outs[-1], queries, *c.device, 0.09, table, i32[0], i32[1], i32[1], 40, 40, None, kind,
+                                            num_parts=parts)
+            # (rows by many: the kernel for long prompts)
+            many = queries.repeat(1, 8, 1)
+            outs.append(torch.empty_like(many))
+            _C.ops.context_attention_scaled(outs[-1], many, *c.device, 0.09, table, i32[0], i32[1], i32[1], 40, 40, None, kind,
+                                            num_parts=parts)
+        results.append([*rows, *outs])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    check_write(Cache(7, heads, size, block, kind), key, value, slots_of(tables, block, [0, 0], lens))
+
+
+def test_read_into_rows_far_apart():
+    """A row of the output every 2^27 bytes, 5 GiB in all."""
+    c = Cache(4, 2, 128, 16, "int8")
+    step = 1 << 26
+    buffer = torch.empty(39 * step + 2 * 128, dtype=torch.bfloat16, device=DEV)
+    far = buffer.as_strided((40, 2, 128), (step, 128, 1))
+    near = [torch.empty(40, 2, 128, dtype=torch.bfloat16, device=DEV) for _ in range(3)]
+    args = [torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([[2, 0, 3]], [0], [40])]
+    _C.cache_ops.gather_cache_scaled(near[0], near[1], *c.device, *args, 40, "int8")
+    _C.cache_ops.gather_cache_scaled(near[2], far, *c.device, *args, 40, "int8")
+    assert torch.equal(far, near[1]) and torch.equal(near[0], near[2])
+    _C.cache_ops.gather_cache_scaled(far, near[2], *c.device, *args, 40, "int8")
+    assert torch.equal(far, near[0]) and torch.equal(near[1], near[2])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size,block", [(64, 16), (80, 8), (128, 16), (128, 32)])
+def test_launches_of_many_workgroups(kind, size, block):
+    """Shapes whose launches differ from the small ones': decode of many pairs, short prompts of many pairs by tiles of 16 rows, long ones
+    by tiles of 256; the first and last sequences and a few heads are looked at."""
+    kv_heads = 64
+    lens = [1150, 40, 9] if block > 8 else [1150, 40]
+    c = Cache(sum((n + block - 1) // block for n in lens) + 1, kv_heads, size, block, kind)
+    tables = tables_for(lens, block, c.key.shape[0])
+    some = [0, 13, 63]
+
+    class Few:
+        kind, key_codes, value_codes = c.kind, c.key_codes[:, :, some], c.value_codes[:, :, some]
+        key_scales, value_scales = c.key_scales[:, some], c.value_scales[:, some]
+
+    # one token each: 8 sequences of 64 heads, most of them the same
+    pick = [1, 1, 1, 1, 1, 1, 1, len(lens) - 1]
+    query = random_query(8, kv_heads, size, torch.float16)
+    got = decode(c, query, tables[pick], [lens[i] for i in pick], size ** -0.5)
+    check_attention(got[:, some], Few, query[:, some], tables[pick], [lens[i] for i in pick], [1] * 8, size ** -0.5)
+    # 100 new tokens of 3 sequences, of which the short ones have fewer tokens than that
+    pick = [0, 1, 1]
+    query = random_query(300, kv_heads, size, torch.bfloat16)
+    got = context(c, query, tables[pick], [0, 100, 200], [100, 30, 40], [1150, 40, 40], size ** -0.5)
+    check_attention(got[:, some], Few, query[:, some], tables[pick], [1150, 40, 40], [100, 30, 40], size ** -0.5, starts=[0, 100, 200])
+    # a whole prompt
+    query = random_query(1150, kv_heads, size, torch.bfloat16)
+    got = context(c, query, tables[:1], [0], [1140], [1150], size ** -0.5)
+    check_attention(got[:, some], Few, query[:, some], tables[:1], [1150], [1140], size ** -0.5)
+    assert (got[1140:] == 7.0).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_scale_below_zero(kind, dtype):
+    lens, new = [300, 70], [120, 3]
+    c = Cache(30, 2, 64, 16, kind)
+    tables = tables_for(lens, 16, 30)
+    query = random_query(123, 4, 64, dtype)
+    check_attention(context(c, query, tables, [0, 120], new, lens, -0.11), c, query, tables, lens, new, -0.11)
+    check_attention(decode(c, query[:2], tables, lens, -0.11), c, query[:2], tables, lens, [1, 1], -0.11)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new", [4, 300])
+def test_graphs_that_share_their_memory(kind, new):
+    """Attention of several new tokens in two captured graphs of one pool, split and whole, replayed in turn with eager work between."""
+    heads, kv_heads, size, block = 4, 2, 128, 16
+    c = Cache(60, kv_heads, size, block, kind)
+    tables = tables_for([800], block, 60).to(DEV)
+    i32 = [torch.zeros(1, dtype=torch.int32, device=DEV) for _ in range(3)]
+    query = torch.zeros(new, heads, size, dtype=torch.bfloat16, device=DEV)
+    outs = [torch.zeros_like(query) for _ in range(3)]
+
+    def run(out, parts):
+        _C.ops.context_attention_scaled(out, query, *c.device, 0.09, tables, *i32, new, 800, None, kind, num_parts=parts)
+
+    i32[1].fill_(new), i32[2].fill_(700)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(outs[2], 1), run(outs[2], 3)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    with torch.inference_mode():
+        with torch.cuda.graph(graphs[0]):
+            run(outs[0], 3)
+        with torch.cuda.graph(graphs[1], pool=graphs[0].pool()):
+            run(outs[1], 1), run(outs[0], 2)
+    for i in range(4):
+        query.copy_(torch.randn(query.shape, generator=torch.Generator().manual_seed(i)))
+        i32[2].fill_(520 + 90 * i)
+        for which, (at, parts) in enumerate(((0, 3), (1, 1))):
+            graphs[which].replay()
+            torch.cuda.synchronize()
+            run(outs[2], parts)
+            assert torch.equal(outs[at], outs[2])
+        run(outs[2], 2)
+        assert torch.equal(outs[0], outs[2])

@@ -104,3 +104,17 @@ def test_blocks_go_with_their_scales(kind):
     for (k, v), old in zip(cache.gpu_cache, before):
         for now, was in zip((k, v, *k.scales), old):
             assert torch.equal(now, was[[1, 1, 4, 1, 4, 4]])
+
+
+def test_copies_of_nothing():
+    from splitwise_amd.config import CacheConfig
+    from splitwise_amd.worker.cache_engine import CacheEngine
+    config = CacheConfig(16, 0.5, 0, "int8")
+    config.num_gpu_blocks, config.num_cpu_blocks = 3, 1
+    model = types.SimpleNamespace(dtype=torch.bfloat16, get_head_size=lambda: 64, get_num_layers=lambda p: 1, get_num_kv_heads=lambda p: 2)
+    cache = CacheEngine(config, model, types.SimpleNamespace(), torch.device("cuda", 0))
+    cache.gpu_scales.uniform_()
+    before = cache.gpu_scales.clone()
+    cache.copy({})
+    cache.copy({1: []})
+    assert torch.equal(cache.gpu_scales, before)

@@ -164,7 +164,7 @@ int sc_attend(const char* what, ScAttention a, int num_seqs, int64_t num_blocks,
   const ScPlan plan = sc_plan(num_seqs, max_new_len, a.heads, a.kv_heads, a.head_size, max_context_len);
   a.tile_rows = plan.tile_rows;
   const int64_t tiles = ((int64_t)max_new_len * a.group + a.tile_rows - 1) / a.tile_rows;
-  SW_CHECK_ARG(tiles * a.kv_heads <= INT32_MAX, "%s: %d new tokens", what, max_new_len);
+  SW_CHECK_ARG(tiles * a.kv_heads <= kScMostWorkgroups && max_new_len <= kScMostWorkgroups, "%s: %d new tokens", what, max_new_len);
   if (num_seqs == 0 || max_new_len == 0 || a.num_rows == 0) return SW_OK;
   a.num_blocks = (int)num_blocks;
   a.tiles = (int)tiles;

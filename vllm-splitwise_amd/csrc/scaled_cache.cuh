@@ -13,6 +13,9 @@ using sc_f16x2 = __attribute__((ext_vector_type(2))) _Float16;
 using sc_u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
 using sc_u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 
+// Workgroups of up to 512 threads that a launch's first dimension can have: it counts threads in 32 bits.
+constexpr int64_t kScMostWorkgroups = UINT32_MAX / 512;
+
 // Blocks whose largest magnitude is below this are held as zeros: its reciprocal, and that of a 448th of it, are finite.
 constexpr float kScTiny = 0x1p-100f;
 

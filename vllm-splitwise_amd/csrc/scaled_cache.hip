@@ -494,7 +494,7 @@ int sw_reshape_and_cache_scaled(const void* key, const void* value, void* key_ca
   w.window = num_tokens <= 1024 ? 1 : kScWindow;
   w.head_pairs = (num_heads + 1) / 2;
   const int64_t workgroups = ((int64_t)num_tokens + w.window - 1) / w.window * w.head_pairs;
-  SW_CHECK_ARG(workgroups <= INT32_MAX, "reshape_and_cache_scaled: %d tokens of %d heads are too many for a call", num_tokens, num_heads);
+  SW_CHECK_ARG(workgroups <= kScMostWorkgroups, "reshape_and_cache_scaled: %d tokens of %d heads are too many for a call", num_tokens, num_heads);
   const dim3 grid((unsigned)workgroups);
   return sc_by_type(act_dtype, cache_dtype, [&](auto a, auto e) {
     return sc_by_size(head_size, block_size, [&](auto bs, auto d) -> int {
@@ -530,8 +530,10 @@ int sw_gather_cache_scaled(void* key, void* value, const void* key_cache, const 
   w.num_blocks = (int)num_blocks, w.width = max_blocks_per_seq, w.heads = num_heads, w.head_size = head_size;
   const int blocks = std::min((int)(((int64_t)max_seq_len + block_size - 1) / block_size), max_blocks_per_seq);
   if (num_seqs == 0 || blocks == 0 || num_rows == 0) return SW_OK;
+  // (a lane's place in a value's row counts 12 rows in 32 bits)
+  SW_CHECK_ARG(num_rows == 1 || value_stride * es < 1 << 28, "gather_cache_scaled: rows of values must lie less than 2^28 bytes apart");
   w.head_pairs = (num_heads + 1) / 2;
-  SW_CHECK_ARG((int64_t)blocks * w.head_pairs <= INT32_MAX, "gather_cache_scaled: sequences of %d blocks of %d heads are too long for a call",
+  SW_CHECK_ARG((int64_t)blocks * w.head_pairs <= kScMostWorkgroups, "gather_cache_scaled: sequences of %d blocks of %d heads are too long for a call",
                blocks, num_heads);
   const dim3 grid(blocks * w.head_pairs, num_seqs);
   return sc_by_type(act_dtype, cache_dtype, [&](auto a, auto e) {

@@ -627,7 +627,7 @@ def reshape_and_cache_scaled(key: torch.Tensor, value: torch.Tensor, key_cache: 
     is rescaled; it starts over with the token for the block's first slot, whose other slots become zeros unless the call writes them.
     Infinities go to the largest code, NaN to 0.  Slots outside the cache (negative: padding) are skipped.  A block's
     tokens may stand anywhere in the list, and of several for one slot the last one stays (unless neighbours in the list fill the whole
-    block in order: then which one does is not specified)."""
+    block in order: then the block may hold either's codes and scale, or some of each)."""
     status = _native.reshape_and_cache_scaled(key, value, key_cache, value_cache, key_scales, value_scales, slot_mapping, kv_cache_dtype)
     if status is not None:
         return _check(status)
