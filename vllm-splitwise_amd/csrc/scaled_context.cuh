@@ -11,6 +11,10 @@
 //     the reference (the largest's, but for 2^6), into the weight's exponent; and its reciprocal, which takes it out of the weights' sum
 //     again.  A score costs one product-and-sum, one exp2, one addition, half a maximum and half a packing;
 //   * sums are rescaled only where a row's maximum has grown by more than 2^8 or a value scale by more than 2^6.
+// Measured: 2041 tokens of 64 heads on 8 behind 14003 (16-bit floats of 128 dims, int8) 1000 us, 1.0 PFLOP/s, where a plain product of
+// large matrices reaches 1.2: matrix cores busy 40 % of the cycles and vector units 60 %, hardly at once, at a clock that the power lets
+// down to 2 GHz.  (So what takes vector instructions out counts, not what moves them: two halves of the waves half a stage apart, with a
+// barrier more, 1135; all products of a stage together and its weights behind them 1125.)  8 x 1024 of 32 heads on 8 behind 1000 353 us.
 #pragma once
 
 #include "scaled_attention.cuh"
@@ -23,7 +27,7 @@ constexpr int kScRows = 32;                                   // of a wave
 constexpr float kScLazy = 8.f;                                // powers of two by which a weight may pass 1
 constexpr float kScHigher = 6.f;                              // and by which a value scale may pass the reference: both fit a half
 constexpr float kScDeep = 40.f;                               // below the reference by more a value scale counts as that much below it
-constexpr float kScLeast = 0x1p-120f;                         // and below this as this (a block of zeros has the scale 0)
+constexpr float kScLeast = 0x1p-110f;                         // and below this as this (a block of zeros has the scale 0, others more)
 
 constexpr int kScSteps = 8;                                   // dwords of codes of a key's piece and a value's
 
@@ -34,6 +38,9 @@ __host__ __device__ constexpr int sc_vstride(int head) { return sc_stage(head) *
 __host__ __device__ constexpr int sc_buffer(int head) {
   return sc_stage(head) * sc_kstride(head) + sc_padded(head) * sc_vstride(head) + 128;      // and the scales
 }
+
+// The larger one; a NaN, if one of them is one.  (One instruction for three, and none to quiet a NaN first.)
+__device__ __forceinline__ float sc_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
 template <bool E4M3, int HEAD, int BS, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScAttention a) {
@@ -196,7 +203,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
     }
   };
 
-  float m_run = -INFINITY, l_run = 0.f, ref_run = -INFINITY;   // (the reference: of the wave, whose rows' sums are in units of 2 to it)
+  float m_run = -INFINITY, l_run = 0.f;
+  float ref_run = -INFINITY, unit = 0.f;                       // the reference, of the wave, whose rows' sums are in units of 2 to it
   sc_f32x16 o[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b)
@@ -239,15 +247,16 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
       const uint32_t missing = __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint32_t*>(f)[24]);
       auto top_of = [&](int b) {
         const int u = b >> 2, i = (b & 3) * 4;
-        return fmaxf(fmaxf(x[u][i], x[u][i + 1]), fmaxf(x[u][i + 2], x[u][i + 3])) * fs[b];
+        return sc_max(sc_max(x[u][i], x[u][i + 1]), sc_max(x[u][i + 2], x[u][i + 3])) * fs[b];
       };
       float top = -INFINITY;
       __builtin_amdgcn_s_setprio(1);
-      // The scores' products, their operands read three ahead; between them the next stage's widening and the maximum of the scores that
+      // The scores' products, their operands read ahead; between them the next stage's widening and the maximum of the scores that
       // are there: the order is held.
       {
         auto operand = [&](int n) { return *reinterpret_cast<const sc_f16x8*>(kp + n / KS * 32 * KSTRIDE + n % KS * 32); };
-        constexpr int N = NT * KS, AHEAD = 3, STEPS = kScSteps * NP;
+        // (heads of 256 have no registers for more than one ahead: 166 us for 2 x 1000 tokens of 4 heads behind 1500, 214 with three and two)
+        constexpr int N = NT * KS, AHEAD = HEAD > 128 ? 1 : 3, STEPS = kScSteps * NP;
         sc_f16x8 ring[AHEAD + 1];
 #pragma unroll
         for (int n = 0; n < AHEAD; ++n) ring[n] = operand(n);
@@ -257,7 +266,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
           x[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ring[n % (AHEAD + 1)], __builtin_bit_cast(sc_f16x8, qf[n % KS]), x[u], 0, 0, 0);
           static_for<STEPS*(n + 1) / N - STEPS * n / N>(
               [&](auto K) { lay_step(std::integral_constant<int, STEPS * n / N + decltype(K)::value>{}, buf ^ 1); });
-          if constexpr (u > 0 && n % KS >= KS - 4) top = fmaxf(top, top_of(4 * u - 4 + n % KS - KS + 4));
+          if constexpr (u > 0 && n % KS >= KS - 4) top = sc_max(top, top_of(4 * u - 4 + n % KS - KS + 4));
           __builtin_amdgcn_sched_barrier(0);
         });
       }
@@ -281,11 +290,12 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
         for (int b = 0; b < SB; ++b) fs[b] = 1.f;
         top = -INFINITY;
 #pragma unroll
-        for (int b = 0; b < SB - 4; ++b) top = fmaxf(top, top_of(b));
+        for (int b = 0; b < SB - 4; ++b) top = sc_max(top, top_of(b));
       }
 #pragma unroll
-      for (int b = SB - 4; b < SB; ++b) top = fmaxf(top, top_of(b));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      for (int b = SB - 4; b < SB; ++b) top = sc_max(top, top_of(b));
+      const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+      top = sc_max(__uint_as_float(both[0]), __uint_as_float(both[1]));
       // (all lanes have the same scales)
       float most_v = log_v[0], least_v = log_v[0];
 #pragma unroll
@@ -297,19 +307,19 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
         l_run *= alpha;
         const float shrink = ref_run == -INFINITY ? 0.f : alpha * __builtin_amdgcn_exp2f(ref_run - ref_new);
         ref_run = ref_new;
+        unit = __builtin_amdgcn_exp2f(ref_run);
 #pragma unroll
         for (int b = 0; b < DB; ++b)
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[b][i] *= shrink;
       }
-      const float unit = __builtin_amdgcn_exp2f(ref_run);
-      float undo[SB];
+      float undo[SB], sum = 0.f;
 #pragma unroll
-      for (int b = 0; b < SB; ++b) undo[b] = f[16 + b] * unit;
+      for (int b = 0; b < SB; ++b) undo[b] = f[16 + b];
       if (__any(least_v < ref_run - kScDeep)) {
 #pragma unroll
         for (int b = 0; b < SB; ++b)
-          if (log_v[b] < ref_run - kScDeep) log_v[b] = ref_run - kScDeep, undo[b] = __builtin_amdgcn_exp2f(kScDeep);
+          if (log_v[b] < ref_run - kScDeep) log_v[b] = ref_run - kScDeep, undo[b] = __builtin_amdgcn_exp2f(kScDeep - ref_run);
       }
       const float base = sc_base(m_run) + ref_run;
       // Weights of a run of 16 tokens, a few between each two products of the run before.
@@ -324,13 +334,13 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
       };
       auto pack = [&](auto N_) {
         constexpr int n = decltype(N_)::value;
-        l_run = fmaf((p[0] + p[1]) + (p[2] + p[3]), undo[2 * n], l_run);
-        l_run = fmaf((p[4] + p[5]) + (p[6] + p[7]), undo[2 * n + 1], l_run);
+        sum = fmaf((p[0] + p[1]) + (p[2] + p[3]), undo[2 * n], sum);
+        sum = fmaf((p[4] + p[5]) + (p[6] + p[7]), undo[2 * n + 1], sum);
 #pragma unroll
         for (int w = 0; w < 4; ++w) pf[w] = sc_pack_f16(p[2 * w], p[2 * w + 1]);
       };
       auto operand = [&](int n) { return *reinterpret_cast<const sc_f16x8*>(vp + n % DB * 32 * VSTRIDE + n / DB * 32); };
-      constexpr int AHEAD = 2;
+      constexpr int AHEAD = HEAD > 128 ? 1 : 2;
       sc_f16x8 ring[AHEAD + 1];
 #pragma unroll
       for (int n = 0; n < AHEAD; ++n) ring[n] = operand(n);
@@ -348,13 +358,13 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
         }
         __builtin_amdgcn_sched_barrier(0);
       });
+      l_run = fmaf(sum, unit, l_run);
     }
     __syncthreads();
   }
 
   l_run += __shfl_xor(l_run, 32, 64);
   if (!real) return;
-  const float unit = ref_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref_run);
   const float inv = a.partial ? unit : l_run > 0.f ? unit / l_run : l_run != l_run ? l_run : 0.f;   // a row that sees nothing gives zeros
   float* to = nullptr;
   uint16_t* out = nullptr;
