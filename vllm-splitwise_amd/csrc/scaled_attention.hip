@@ -126,10 +126,10 @@ ScPlan sc_plan(int num_seqs, int max_new_len, int num_heads, int num_kv_heads, i
     p.waves = head_size <= 128 && w <= (max_context_len >= 4096 && rows <= 16 ? 1024 : 256) ? 8 : 4;
     p.parts = (int)std::min<int64_t>(max_context_len < 1024 ? 1 : ((int64_t)max_context_len + 255) / 256, 256 / w);
   } else {
-    // 256 rows where there are enough of them: half the widening a row (us, 128 / 256 rows: 2041 tokens of 8 heads behind 14003 1127 /
-    // 1040, 8 x 1024 behind 1000 372 / 372, 6 x 301 89 / 87, 30 x 50 behind 10 35 / 39; heads of 64 153 / 169, of 256 554 / 563).
-    // Fewer: parts, for whose sums each row costs 2 x 4 bytes a dim and part (500 tokens of 32 heads behind 4000, 1 / 2 / 4 / 8 parts: 138 / 88 /
-    // 70 / 83; 1000 of 32 heads behind 100, 1 / 2: 46 / 53).
+    // 256 rows where there are enough of them: half the widening a row (us, 128 / 256 rows: 2041 tokens of 8 heads behind 14003 1063 / 998,
+    // 8 x 1024 behind 1000 331 / 325, 6 x 301 78 / 80, 30 x 50 behind 10 33 / 37; heads of 64, 8 x 1024, 212 / 248).
+    // Fewer: parts, for whose sums each row costs 2 x 4 bytes a dim and part (500 tokens of 32 heads behind 4000, 1 / 2 / 4 parts: 111 / 75 /
+    // 67; 1000 of 32 heads behind 100, 1 / 2: 39 / 51; 6 x 301 78 / 108).
     const int64_t w = workgroups(128);
     p.tile_rows = head_size >= 80 && head_size <= 128 && w >= 512 && max_context_len >= 1024 ? 256 : 128;
     p.waves = p.tile_rows / 32;

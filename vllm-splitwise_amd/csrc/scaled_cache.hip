@@ -114,7 +114,9 @@ constexpr int kScLook = 16;          // entries that a thread asks for at a time
 
 // Bound by vector instructions as much as by memory (an element is 2 bytes in and 1 out), so: a lane's addresses are one number and what
 // the compiler can put into the instructions; magnitudes two at a time; codes of finite values, the rule, in 4 instructions an element; and
-// blocks that the call fills look at no single token.
+// blocks that the call fills look at no single token.  5 prompts of some 400 tokens, 32 heads of 128, f16 to e4m3 15.6 us, 16384 tokens of 8 heads
+// in whole blocks 22 us, 4.5 TB/s; 64 single tokens of 32 heads 6.7 us, of which the kernel's own chain of loads (list, list, token) is most.
+// Asking for a short list and for what a block holds earlier made the chain shorter and the rest slower: 0.1 us more there, 1 us more for prompts.
 
 // A lane's pieces are 16 elements of the key of one token, the same for all its pieces: 32 bytes in (64 of fp32), 16 out, where a wave's lie
 // side by side.  FULL: tokens first, first + 1, ... fill the block.

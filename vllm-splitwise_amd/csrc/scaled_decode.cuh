@@ -19,6 +19,11 @@
 // what bf16's 2^-9 or f16's 2^-12 rounding of the result leaves), relative to the largest value scale met so far, which goes into the
 // sums as the maximum does: p sv / r is at most 1 whatever the scales are.  bf16 queries go into halves by a power of two for each row
 // that brings their largest to 2^14 .. 2^15, which goes into the row's scale.
+//
+// Measured (heads of 128): 61 sequences of some 1090 tokens, 32 heads, e4m3, 544 MB, 106 us, 5.2 TB/s, what a large copy reads and
+// writes; 201 of some 2000, 64 heads on 8, int8, 820 MB, 170 us, 4.8 TB/s (of one length 5.4: the longest
+// sequences' workgroups run on alone); 3 of 34000 to 90000, 64 on 8, e4m3 in ten parts and their join, 431 MB, 84 us, 5.1 TB/s; one sequence of 500
+// 8.8 us, a chain of loads.  Two to four tiles of rows a wave, loads a group ahead and pairs of waves that share a group's dims were no faster.
 #pragma once
 
 #include "scaled_attention.cuh"
