@@ -128,12 +128,15 @@ ScPlan sc_plan(int num_seqs, int max_new_len, int num_heads, int num_kv_heads, i
   } else {
     // 256 rows where there are enough of them: half the widening a row (us, 128 / 256 rows: 2041 tokens of 8 heads behind 14003 1063 / 998,
     // 8 x 1024 behind 1000 331 / 325, 6 x 301 78 / 80, 30 x 50 behind 10 33 / 37; heads of 64, 8 x 1024, 212 / 248).
-    // Fewer: parts, for whose sums each row costs 2 x 4 bytes a dim and part (500 tokens of 32 heads behind 4000, 1 / 2 / 4 parts: 111 / 75 /
-    // 67; 1000 of 32 heads behind 100, 1 / 2: 39 / 51; 6 x 301 78 / 108).
+    // Fewer than the 512 that run at once: parts, for whose sums each row costs 2 x 4 bytes a dim and part; short ones up to 256 workgroups, which
+    // have few rows, and long ones up to 512 (us by parts: 120 tokens of 8 heads behind 3000 1 78.5, 4 30.7, 16 25.0, 48 25.2; behind 800 1 32.6,
+    // 4 21.7, 12 21.5; 2 x 42 of 8 heads of 256 on 2 behind 2049 1 320, 3 125, 16 44, 32 41; 400 of 32 on 8 behind 12000 1 282, 4 120, 6 133, 12 142;
+    // 500 of 32 behind 4000 1 110, 2 76, 4 67, 8 78; 512 of 64 on 8 behind 8000 1 198, 2 180, 4 185; 800 behind 600 1 51, 2 77; 1000 of 32 heads
+    // behind 100 1 39, 2 51).
     const int64_t w = workgroups(128);
     p.tile_rows = head_size >= 80 && head_size <= 128 && w >= 512 && max_context_len >= 1024 ? 256 : 128;
     p.waves = p.tile_rows / 32;
-    p.parts = w >= 512 ? 1 : (int)std::min<int64_t>(max_context_len / 768, (512 + w / 2) / w);
+    p.parts = (int)std::max(std::min<int64_t>(max_context_len / 192, 256 / w), std::min<int64_t>(max_context_len / 768, 512 / w));
   }
   p.parts = std::max(1, std::min(p.parts, kScMostParts));
   return p;
