@@ -11,8 +11,8 @@
 //     the reference (the largest's, but for 2^6), into the weight's exponent; and its reciprocal, which takes it out of the weights' sum
 //     again.  A score costs one product-and-sum, one exp2, one addition, half a maximum and half a packing;
 //   * sums are rescaled only where a row's maximum has grown by more than 2^8 or a value scale by more than 2^6.
-// Measured: 2041 tokens of 64 heads on 8 behind 14003 (16-bit floats of 128 dims, int8) 1000 us, 1.0 PFLOP/s, where a plain product of
-// large matrices reaches 1.2: matrix cores busy 40 % of the cycles and vector units 60 %, hardly at once, at a clock that the power lets
+// Measured: 2041 tokens of 64 heads of 128 on 8 behind 14003, bf16, int8, 1000 to 1020 us, 1.0 PFLOP/s, where a plain product of
+// large matrices reaches 1.2: matrix cores busy 48 % of the cycles and vector units 58 %, at a clock that the power lets
 // down to 2 GHz.  (So what takes vector instructions out counts, not what moves them: two halves of the waves half a stage apart, with a
 // barrier more, 1135; all products of a stage together and its weights behind them 1125.)  8 x 1024 of 32 heads on 8 behind 1000 325 us.
 #pragma once
