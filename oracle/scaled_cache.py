@@ -76,7 +76,9 @@ def attention(query, key_codes, value_codes, key_scales, value_scales, table, le
     """query [rows, heads, D], row j at position first + j of a sequence of `length` tokens.  (out, bound): in 64 bits, and how far a
     kernel may be off that keeps scores, sums and weights in 32 bits and hands the second product its weights as halves:
 
-      weights:  relative 2^-11 (a half's rounding), or 2^-25 of the largest value scale below a half's range, and 2^-22 for exp2;
+      weights:  relative 2^-11 (a half's rounding); below a half's normal numbers 2^-25, where the largest product of weight and scale that
+                the row sees stands at 2^7 or above, so 2^-32 of that one; and 2^-22 for exp2;
+      scales:   they go into the exponent as logarithms, 4 roundings of numbers up to 32 and the largest of them, in numerator and sum;
       scores:   the D products and their sum, relative 2^-24 each of sum |q||k|, and three roundings of the score: d; a weight over the
                 sum of weights is then off by 2 d;
       sums:     one rounding for each of T tokens, the running maximum's factors among them, of numerator and denominator.
@@ -97,7 +99,8 @@ def attention(query, key_codes, value_codes, key_scales, value_scales, table, le
     if window:
         see &= at[None] > pos[:, None] - window
     u32 = 2.0 ** -24
-    used = [b for b in table.tolist()[:(length + key_codes.shape[1] - 1) // key_codes.shape[1]] if 0 <= b < key_codes.shape[0]]
+    pages = [b if 0 <= b < key_codes.shape[0] else 0 for b in table.tolist()[:(length + key_codes.shape[1] - 1) // key_codes.shape[1]]]
+    scale_of = value_scales.double()[pages].repeat_interleave(key_codes.shape[1], 0)[:t]          # [tokens, kv heads]
     for h in range(heads):
         g = h // group
         kk, vv = torch.where(there[:, None], k[:, g], 0.0), torch.where(there[:, None], v[:, g], 0.0)
@@ -112,6 +115,8 @@ def attention(query, key_codes, value_codes, key_scales, value_scales, table, le
         w = torch.where(see.any(1, keepdim=True), w, 0.0)
         out[:, h] = w @ vv
         mass = w @ vv.abs()
-        largest = max((float(value_scales[b, g]) for b in used), default=0.0) * TOP[kind]
-        bound[:, h] = mass * (2.0 ** -11 + 2.0 ** -21 + 2 * off + 4 * t * u32) + t * 2.0 ** -25 * largest
+        sv = torch.where(see, scale_of[:, g], 0.0)
+        largest = (w * sv).amax(1, keepdim=True) * TOP[kind]
+        powers = torch.where(sv > 0, sv, 1.0).log2().abs().amax(1, keepdim=True) + 32
+        bound[:, h] = mass * (2.0 ** -11 + 2.0 ** -21 + 2 * off + 2.0 ** -21 * powers + 4 * t * u32) + t * 2.0 ** -32 * largest
     return out, bound

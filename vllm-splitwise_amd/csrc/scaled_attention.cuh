@@ -9,12 +9,13 @@ using sc_f32x4 = __attribute__((ext_vector_type(4))) float;
 using sc_f16x8 = __attribute__((ext_vector_type(8))) _Float16;
 
 struct ScAttention {
-  void* out;                       // [rows, heads, head_size], or null: parts go to the workspace
+  void* out;                       // [rows, heads, head_size]
   const void* query;
   const uint8_t *key_cache, *value_cache;
   const float *key_scales, *value_scales, *slopes;
   const int32_t *tables, *starts, *new_lens, *lens;      // starts null: sequence i has one new token, in row i
-  float* partial;                  // [rows, heads, parts, head_size + 4]: sums, their maximum (powers of two), the weights' sum
+  float* partial;                  // null or the workspace, which then takes the sums: [rows, heads, parts, head_size + 4], sums, the
+                                   // scores' maximum (powers of two), the weights' sum
   int64_t q_stride, out_stride, num_rows, table_stride;
   int num_blocks, width, heads, kv_heads, group, head_size;
   int window;                      // 0: none
@@ -69,6 +70,15 @@ __device__ __forceinline__ int sc_part_end(const ScAttention& a, const ScSequenc
   const int end = min(s.len, pos_high + 1);
   return part == a.parts - 1 ? end : min(end, (part + 1) * a.part_tokens);
 }
+
+// A value scale as a power of two.  Below 2^-110 it is that of a block of zeros: further down than any sum reaches.
+constexpr float kScLeast = 0x1p-110f, kScNone = -300.f;
+__device__ __forceinline__ float sc_log_scale(float s) {
+  return s < kScLeast ? kScNone : __builtin_amdgcn_logf(s);  // (a NaN stays one)
+}
+// A value scale further below the row's reference than this counts as that far below it: its weights are 0 as halves either way, and
+// their sum, brought back by the scale, is still far from the smallest number.
+constexpr float kScDeep = 80.f;
 
 // exp2 of the difference to the running maximum, which is minus infinity while nothing has been seen
 __device__ __forceinline__ float sc_base(float m) { return m == -INFINITY ? 0.f : m; }

@@ -7,10 +7,11 @@
 //     v_mfma_f32_32x32x16_f16: S^T = K . Q^T [32 tokens x 32 rows], O^T += V^T . P^T [32 dims x 32 rows].  A row is a lane's column in both;
 //   * the accumulator of S^T is P^T's operand as it stands: lane half h has tokens 8 b + 4 h + j, so values are laid down with the tokens of
 //     a run of 16 in the order 0-3, 8-11, 4-7, 12-15;
-//   * scales come as three numbers for each 8 tokens, made by 8 threads for all: the key scale; log2 of the value scale, which goes, less
-//     the reference (the largest's, but for 2^6), into the weight's exponent; and its reciprocal, which takes it out of the weights' sum
-//     again.  A score costs one product-and-sum, one exp2, one addition, half a maximum and half a packing;
-//   * sums are rescaled only where a row's maximum has grown by more than 2^8 or a value scale by more than 2^6.
+//   * scales come as three numbers for each 8 tokens, made by 8 threads for all: the key scale; log2 of the value scale, which goes into
+//     the weight's exponent; and its reciprocal, which takes it out of the weights' sum again.  A score costs one product-and-sum, one
+//     exp2, one addition, half a maximum and half a packing;
+//   * sums are rescaled only where a row's maximum or its reference may have grown by more than 2^8: the largest score and the largest
+//     value scale of a stage say so, and only then is looked for the largest of both together.
 // Measured: 2041 tokens of 64 heads of 128 on 8 behind 14003, bf16, int8, 1000 to 1020 us, 1.0 PFLOP/s, where a plain product of
 // large matrices reaches 1.2: matrix cores busy 48 % of the cycles and vector units 58 %, at a clock that the power lets
 // down to 2 GHz.  (So what takes vector instructions out counts, not what moves them: two halves of the waves half a stage apart, with a
@@ -24,10 +25,10 @@ namespace sw {
 using sc_f32x16 = __attribute__((ext_vector_type(16))) float;
 
 constexpr int kScRows = 32;                                   // of a wave
-constexpr float kScLazy = 8.f;                                // powers of two by which a weight may pass 1
-constexpr float kScHigher = 6.f;                              // and by which a value scale may pass the reference: both fit a half
-constexpr float kScDeep = 40.f;                               // below the reference by more a value scale counts as that much below it
-constexpr float kScLeast = 0x1p-110f;                         // and below this as this (a block of zeros has the scale 0, others more)
+constexpr float kScLazy = 8.f;                                // powers of two by which a row's maximum may pass what its sums are to
+constexpr float kScRaised = 7.f;                              // and that its largest weight then stands above 1: 2^15 at most fits a half
+
+constexpr float kScApart = 90.f;                              // powers of two by which that reference and the scores' maximum may be apart
 
 constexpr int kScSteps = 8;                                   // dwords of codes of a key's piece and a value's
 
@@ -42,8 +43,20 @@ __host__ __device__ constexpr int sc_buffer(int head) {
 // The larger one; a NaN, if one of them is one.  (One instruction for three, and none to quiet a NaN first.)
 __device__ __forceinline__ float sc_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
+// The larger and the smaller of a lane's number and another lane's (a register's lanes crossed as CTRL says).
+template <int CTRL>
+__device__ __forceinline__ void sc_most_least(float& most, float& least) {
+  most = fmaxf(most, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(most), CTRL, 0xf, 0xf, true)));
+  least = fminf(least, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(least), CTRL, 0xf, 0xf, true)));
+}
+
+// Waves of a SIMD that the registers are shared out for.  (Two for heads of 256 leave some 50 of a lane's numbers in memory: 2 x 1000 tokens of
+// 4 heads behind 1500 115 us, 81 with one.  Heads of 64 need 2 registers more than three waves have: 8 x 1024 tokens of 32 heads on 8 behind
+// 1000 265 us with two waves, 220 with three and those 2 in memory.)
+__host__ __device__ constexpr int sc_waves(int head, int waves) { return head > 128 ? 1 : head == 64 && waves == 4 ? 3 : 2; }
+
 template <bool E4M3, int HEAD, int BS, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScAttention a) {
+__global__ void __launch_bounds__(WAVES * 64, sc_waves(HEAD, WAVES)) scaled_context_kernel(const ScAttention a) {
   using C = ScCode<E4M3>;
   constexpr int TILE = WAVES * kScRows;
   constexpr int KT = sc_stage(HEAD), NT = KT / 32, KS = HEAD / 16, DB = sc_padded(HEAD) / 32;
@@ -190,21 +203,26 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
     }
   };
   auto lay = [&](int buf) { static_for<kScSteps * NP>([&](auto K) { lay_step(K, buf); }); };
-  // eight tokens' key scale, log2 of the value scale, its reciprocal; and which eights do not exist
+  // eight tokens' key scale, log2 of the value scale, its reciprocal (finite, and of no use where the scale is that of zeros); which eights
+  // do not exist, the largest and the least logarithm
   auto lay_scales = [&](int buf) {
     if (tid < SB) {
       float* f = reinterpret_cast<float*>(smem + buf * BUFFER + KT * KSTRIDE + sc_padded(HEAD) * VSTRIDE);
-      const float v = fmaxf(vscale, kScLeast);
       f[tid] = kscale;
-      f[8 + tid] = vscale != vscale ? vscale : __builtin_amdgcn_logf(v);      // (a NaN of a scale reaches the rows that see its block)
-      f[16 + tid] = __builtin_amdgcn_rcpf(v);
+      float most = sc_log_scale(vscale), least = most;
+      f[8 + tid] = most;
+      f[16 + tid] = __builtin_amdgcn_rcpf(fmaxf(vscale, kScLeast));
       const uint64_t missing = __ballot(!sgood);
-      if (tid == 0) reinterpret_cast<uint32_t*>(f)[24] = (uint32_t)(missing & ((1u << SB) - 1u));
+      sc_most_least<0xB1>(most, least);                        // of the neighbour, of the next two, of the other four
+      sc_most_least<0x4E>(most, least);
+      if constexpr (SB == 8) sc_most_least<0x141>(most, least);
+      if (tid == 0) reinterpret_cast<uint32_t*>(f)[24] = (uint32_t)(missing & ((1u << SB) - 1u)), f[25] = most, f[26] = least;
     }
   };
 
   float m_run = -INFINITY, l_run = 0.f;
-  float ref_run = -INFINITY, unit = 0.f;                       // the reference, of the wave, whose rows' sums are in units of 2 to it
+  float y_run = -INFINITY, unit = 0.f;                         // what the row's sums are powers of two to; 2^(it - m_run)
+  float low = -INFINITY;                                       // a value scale that is none of the weights' sum as it stands
   sc_f32x16 o[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b)
@@ -244,6 +262,7 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
       float fs[SB], log_v[SB];
 #pragma unroll
       for (int b = 0; b < SB; ++b) fs[b] = f[b] * row_scale, log_v[b] = f[8 + b];
+      const float most_v = f[25], least_v = f[26];
       const uint32_t missing = __builtin_amdgcn_readfirstlane(reinterpret_cast<const uint32_t*>(f)[24]);
       auto top_of = [&](int b) {
         const int u = b >> 2, i = (b & 3) * 4;
@@ -286,42 +305,54 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
             const bool see = t <= pos && (a.window <= 0 || t > pos - a.window) && !(missing >> b & 1u);
             x[u][i] = see ? v : -INFINITY;
           }
-#pragma unroll
-        for (int b = 0; b < SB; ++b) fs[b] = 1.f;
         top = -INFINITY;
 #pragma unroll
-        for (int b = 0; b < SB - 4; ++b) top = sc_max(top, top_of(b));
+        for (int b = 0; b < SB; ++b) {
+          fs[b] = 1.f;
+          const float t = top_of(b);
+          if (t == -INFINITY) log_v[b] = 0.f;                  // (of a block that the row sees nothing of not even a NaN counts)
+          top = sc_max(top, t);
+        }
+      } else {
+#pragma unroll
+        for (int b = SB - 4; b < SB; ++b) top = sc_max(top, top_of(b));
       }
+      auto of_both = [](float v) {
+        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        return sc_max(__uint_as_float(both[0]), __uint_as_float(both[1]));
+      };
+      top = of_both(top);
+      if (__any(top > m_run + kScLazy || top + most_v > y_run + (kScLazy + kScRaised))) {
+        float y_top = -INFINITY;
 #pragma unroll
-      for (int b = SB - 4; b < SB; ++b) top = sc_max(top, top_of(b));
-      const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-      top = sc_max(__uint_as_float(both[0]), __uint_as_float(both[1]));
-      // (all lanes have the same scales)
-      float most_v = log_v[0], least_v = log_v[0];
-#pragma unroll
-      for (int b = 1; b < SB; ++b) most_v = fmaxf(most_v, log_v[b]), least_v = fminf(least_v, log_v[b]);
-      if (__any(top > m_run + kScLazy || most_v > ref_run + kScHigher)) {
-        const float m_new = fmaxf(m_run, top), ref_new = most_v > ref_run + kScHigher ? most_v : ref_run;
-        const float alpha = __builtin_amdgcn_exp2f(m_run - sc_base(m_new));
-        m_run = m_new;
-        l_run *= alpha;
-        const float shrink = ref_run == -INFINITY ? 0.f : alpha * __builtin_amdgcn_exp2f(ref_run - ref_new);
-        ref_run = ref_new;
-        unit = __builtin_amdgcn_exp2f(ref_run);
+        for (int b = 0; b < SB; ++b) y_top = sc_max(y_top, top_of(b) + log_v[b]);
+        const float m_new = fmaxf(m_run, top), y_new = fmaxf(y_run, of_both(y_top) - kScRaised);
+        l_run *= __builtin_amdgcn_exp2f(m_run - sc_base(m_new));
+        const float shrink = __builtin_amdgcn_exp2f(y_run - sc_base(y_new)), gap = sc_base(y_new) - sc_base(m_new);
+        m_run = m_new, y_run = y_new;
+        unit = __builtin_amdgcn_exp2f(gap);
+        low = fabsf(gap) <= kScApart ? fmaxf(gap - kScDeep, kScNone + 1.f) : INFINITY;
 #pragma unroll
         for (int b = 0; b < DB; ++b)
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[b][i] *= shrink;
       }
+      // Scales far below the row's largest, or all of them far from 1: the weights' sum is the scores', and what is far below is no weight.
+      const bool apart = __any(least_v < low);
+      float direct = 0.f;
+      if (apart) {
+        const float m_base = sc_base(m_run), deep = sc_base(y_run) - m_base - kScDeep;
+#pragma unroll
+        for (int b = 0; b < SB; ++b) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) direct += __builtin_amdgcn_exp2f(fmaf(x[b >> 2][(b & 3) * 4 + i], fs[b], -m_base));
+          if (log_v[b] < deep) log_v[b] = -INFINITY;
+        }
+      }
       float undo[SB], sum = 0.f;
 #pragma unroll
       for (int b = 0; b < SB; ++b) undo[b] = f[16 + b];
-      if (__any(least_v < ref_run - kScDeep)) {
-#pragma unroll
-        for (int b = 0; b < SB; ++b)
-          if (log_v[b] < ref_run - kScDeep) log_v[b] = ref_run - kScDeep, undo[b] = __builtin_amdgcn_exp2f(kScDeep - ref_run);
-      }
-      const float base = sc_base(m_run) + ref_run;
+      const float base = sc_base(y_run);
       // Weights of a run of 16 tokens, a few between each two products of the run before.
       const char* vp = v_img + col * VSTRIDE + half * 16;
       constexpr int RN = 2 * NT;
@@ -358,14 +389,15 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
         }
         __builtin_amdgcn_sched_barrier(0);
       });
-      l_run = fmaf(sum, unit, l_run);
+      l_run = apart ? l_run + direct : fmaf(sum, unit, l_run);
     }
     __syncthreads();
   }
 
   l_run += __shfl_xor(l_run, 32, 64);
   if (!real) return;
-  const float inv = a.partial ? unit : l_run > 0.f ? unit / l_run : l_run != l_run ? l_run : 0.f;   // a row that sees nothing gives zeros
+  // (the two factors one after the other: their product may be below the smallest number)
+  const float inv = a.partial ? 1.f : l_run > 0.f ? 1.f / l_run : l_run != l_run ? l_run : 0.f;   // a row that sees nothing gives zeros
   float* to = nullptr;
   uint16_t* out = nullptr;
   if (a.partial) {
@@ -383,7 +415,8 @@ __global__ void __launch_bounds__(WAVES * 64, 2) scaled_context_kernel(const ScA
     for (int q = 0; q < 4; ++q) {
       const int d = 32 * b + 8 * q + 4 * half;
       if (HEAD % 32 != 0 && d >= HEAD) continue;
-      const float v0 = o[b][4 * q] * inv, v1 = o[b][4 * q + 1] * inv, v2 = o[b][4 * q + 2] * inv, v3 = o[b][4 * q + 3] * inv;
+      const float v0 = o[b][4 * q] * unit * inv, v1 = o[b][4 * q + 1] * unit * inv, v2 = o[b][4 * q + 2] * unit * inv,
+                  v3 = o[b][4 * q + 3] * unit * inv;
       if (a.partial) *reinterpret_cast<sc_f32x4*>(to + d) = sc_f32x4{v0, v1, v2, v3};
       else *reinterpret_cast<sc_u32x2*>(out + d) = sc_u32x2{sc_pack16(v0, v1, a.bf16), sc_pack16(v2, v3, a.bf16)};
     }

@@ -15,10 +15,13 @@
 //     Q.K  slot (kq, e) of step 2 m + h  <->  dim 64 m + 16 kq + 8 h + e
 //     S tile j of lane (kq, row), i      <->  token 4 j + i of run kq: 16 weights, which are
 //     P.V  slot (kq, e) of step h        <->  token 8 h + e of run kq
-// Scales are a factor of the score and of the weight, both fp32.  The weights go to the second product as halves (an error of 2^-12, under
-// what bf16's 2^-9 or f16's 2^-12 rounding of the result leaves), relative to the largest value scale met so far, which goes into the
-// sums as the maximum does: p sv / r is at most 1 whatever the scales are.  bf16 queries go into halves by a power of two for each row
-// that brings their largest to 2^14 .. 2^15, which goes into the row's scale.
+// Scales are a factor of the score and, as powers of two, a summand of the weight's exponent, both fp32:
+//     w_t = 2^(x_t + log2 sv_t - y),   sum_t p_t = sum_t w_t 2^(y - log2 sv_t),     x_t the score in powers of two
+// w_t goes to the second product as a half, rounded by at most 2^-11 of it (f16's own step, an eighth of bf16's), where y is kept 14 below
+// the largest exponent that the ROW has met: its largest weight is 2^14 whatever blocks without a token for it hold, and what a half cannot
+// hold as a normal number is 2^-28 of that.  (A reference of scores and one of scales apart would let a large scale that has no weight take
+// the bits of all others.)  bf16 queries go into halves by a power of two for each row that brings their largest to 2^14 .. 2^15, which goes
+// into the row's scale.
 //
 // Measured (heads of 128): 61 sequences of some 1090 tokens, 32 heads, e4m3, 544 MB, 106 us, 5.2 TB/s, what a large copy reads and
 // writes; 201 of some 2000, 64 heads on 8, int8, 820 MB, 170 us, 4.8 TB/s (of one length 5.4: the longest
@@ -29,6 +32,8 @@
 #include "scaled_attention.cuh"
 
 namespace sw {
+
+constexpr float kScUp = 14.f, kScDown = 0x1p-14f;             // powers of two that a row's largest weight stands above 1, and back
 
 // NW waves take the groups of 64 tokens of one (sequence, kv head, tile of 16 rows, part) in turn and join at the end.
 // EXACT: head_size == HEAD; else it is a smaller multiple of 16 (dims behind it count as zeros).
@@ -106,7 +111,8 @@ __global__ void __launch_bounds__(NW * 64, HEAD <= 128 ? 2 : 1) scaled_decode_ke
   const int64_t head_bytes = (int64_t)head_size * BS;
   const int32_t* table = a.tables + (int64_t)seq * a.table_stride;
 
-  float m_run = -INFINITY, l_run = 0.f, r_run = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;                       // the scores' maximum, the sum of 2^(score - it)
+  float y_run = -INFINITY;                                    // and what the sums `acc` are powers of two to
   sc_f32x4 acc[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) acc[dt] = sc_f32x4{0.f, 0.f, 0.f, 0.f};
@@ -180,10 +186,13 @@ __global__ void __launch_bounds__(NW * 64, HEAD <= 128 ? 2 : 1) scaled_decode_ke
     good &= left >= 16 ? 0xffffu : left <= 0 ? 0u : (1u << left) - 1u;
     // (wave-uniform) all 64 tokens are there and every row sees all of them
     const bool masked = tok0 + 64 > all_see || tok0 < none_hidden || __any(good != 0xffffu);
-    float gmax = -INFINITY;
+    float top[PB];
+#pragma unroll
+    for (int b = 0; b < PB; ++b) top[b] = -INFINITY;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float f = row_scale * ks[PB == 2 ? j >> 1 : 0];
+      const int b = PB == 2 ? j >> 1 : 0;
+      const float f = row_scale * ks[b];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int t = run0 + 4 * j + i;
@@ -194,40 +203,46 @@ __global__ void __launch_bounds__(NW * 64, HEAD <= 128 ? 2 : 1) scaled_decode_ke
           v = see ? v : -INFINITY;
         }
         x[j][i] = v;
-        gmax = fmaxf(gmax, v);
+        top[b] = fmaxf(top[b], v);
       }
     }
-    float smax = 0.f;
+    float gmax = -INFINITY, ymax = -INFINITY, lv[PB];
 #pragma unroll
     for (int b = 0; b < PB; ++b) {
-      if (masked && (PB == 1 ? good == 0 : (good >> (8 * b) & 0xffu) == 0)) vs[b] = 0.f;
-      smax = fmaxf(smax, vs[b]);
+      // (of a block that the row sees nothing of not even a NaN counts)
+      lv[b] = top[b] == -INFINITY ? 0.f : sc_log_scale(vs[b]);
+      gmax = fmaxf(gmax, top[b]);
+      ymax = fmaxf(ymax, top[b] + lv[b]);
     }
     gmax = fmaxf(gmax, __shfl_xor(gmax, 16, 64));
     gmax = fmaxf(gmax, __shfl_xor(gmax, 32, 64));
-    smax = fmaxf(smax, __shfl_xor(smax, 16, 64));
-    smax = fmaxf(smax, __shfl_xor(smax, 32, 64));
+    ymax = fmaxf(ymax, __shfl_xor(ymax, 16, 64));
+    ymax = fmaxf(ymax, __shfl_xor(ymax, 32, 64));
     const float m_new = fmaxf(m_run, gmax), base = sc_base(m_new);
-    const float r_new = fmaxf(r_run, smax), r_inv = r_new > 0.f ? 1.f / r_new : 0.f;
-    const float alpha = __builtin_amdgcn_exp2f(m_run - base);
+    const float y_new = fmaxf(y_run, ymax - kScUp), y_base = sc_base(y_new), gap = y_base - base;
+    const float alpha = __builtin_amdgcn_exp2f(m_run - base), shrink = __builtin_amdgcn_exp2f(y_run - y_base);
     m_run = m_new;
-    const float shrink = alpha * (r_run * r_inv);
-    r_run = r_new;
+    y_run = y_new;
 
     // ---- weights: their sum, and as the second product takes them
     sc_u32x4 pf[2];
-    float sum = 0.f;
+    float sum = 0.f, shift[PB], undo[PB];
+#pragma unroll
+    for (int b = 0; b < PB; ++b) {
+      const float low = gap - kScDeep;                        // (a weight of that is 0 as a half, and in `sum` it still counts)
+      const float l = lv[b] < low ? low : lv[b];
+      shift[b] = l - gap;
+      undo[b] = __builtin_amdgcn_exp2f(gap - l);
+    }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float f = vs[PB == 2 ? j >> 1 : 0] * r_inv;
+      const int b = PB == 2 ? j >> 1 : 0;
       float p[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(x[j][i] - base);
-        sum += p[i];
-      }
-      pf[j >> 1][2 * (j & 1)] = sc_pack_f16(p[0] * f, p[1] * f);
-      pf[j >> 1][2 * (j & 1) + 1] = sc_pack_f16(p[2] * f, p[3] * f);
+      for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f((x[j][i] - base) + shift[b]);
+      sum = fmaf((p[0] + p[1]) + (p[2] + p[3]), undo[b], sum);
+      pf[j >> 1][2 * (j & 1)] = sc_pack_f16(p[0], p[1]);
+      pf[j >> 1][2 * (j & 1) + 1] = sc_pack_f16(p[2], p[3]);
     }
     l_run = l_run * alpha + sum;
 #pragma unroll
@@ -267,9 +282,10 @@ __global__ void __launch_bounds__(NW * 64, HEAD <= 128 ? 2 : 1) scaled_decode_ke
   const float base = sc_base(m_all);
 #pragma unroll
   for (int w = 0; w < NW; ++w) l_all += stat[w * 32 + 16 + r] * __builtin_amdgcn_exp2f(stat[w * 32 + r] - base);
-  const float mine = __builtin_amdgcn_exp2f(m_run - base) * r_run;
+  // (in steps: all in one may be below the smallest number)
+  const float mine = __builtin_amdgcn_exp2f(m_run - base) * __builtin_amdgcn_exp2f(y_run + kScUp - sc_base(m_run));
 #pragma unroll
-  for (int dt = 0; dt < DT; ++dt) acc[dt] *= mine;
+  for (int dt = 0; dt < DT; ++dt) acc[dt] = acc[dt] * kScDown * mine;
 #pragma unroll
   for (int half = NW / 2; half >= 1; half >>= 1) {
     if (wave >= half && wave < 2 * half) {
