@@ -213,3 +213,13 @@ def test_scales_count_in_a_block():
     size = lambda kind: CacheEngine.get_cache_block_size(16, kind, model, None)  # noqa: E731
     assert size("auto") == 3 * 2 * 16 * 2 * 64 * 2 and size("fp8_e5m2") == size("auto") // 2
     assert size("int8") == size("fp8_e4m3") == size("fp8_e5m2") + 3 * 2 * 2 * 4
+
+
+def test_every_kernel_that_is_built_is_launched():
+    """Workgroups of eight waves exist for heads of 80 to 128, which the launch rule gives them to, and for no others."""
+    import re
+    with open(_C.library_path(), "rb") as f:
+        names = set(re.findall(rb"scaled_context_kernelILb([01])ELi(\d+)ELi(\d+)ELi(\d+)E", f.read()))
+    built = {(int(e), int(head), int(block), int(waves)) for e, head, block, waves in names}
+    assert built == {(e, head, block, waves) for e in (0, 1) for block in (8, 16, 32) for waves in (4, 8)
+                     for head in ((64, 80, 96, 112, 128, 256) if waves == 4 else (80, 96, 112, 128))}

@@ -53,10 +53,10 @@ __device__ __forceinline__ void sc_most_least(float& most, float& least) {
 // Waves of a SIMD that the registers are shared out for.  (Two for heads of 256 leave some 50 of a lane's numbers in memory: 2 x 1000 tokens of
 // 4 heads behind 1500 115 us, 81 with one.  Heads of 64 need 2 registers more than three waves have: 8 x 1024 tokens of 32 heads on 8 behind
 // 1000 265 us with two waves, 220 with three and those 2 in memory.)
-__host__ __device__ constexpr int sc_waves(int head, int waves) { return head > 128 ? 1 : head == 64 && waves == 4 ? 3 : 2; }
+__host__ __device__ constexpr int sc_waves(int head) { return head > 128 ? 1 : head == 64 ? 3 : 2; }
 
 template <bool E4M3, int HEAD, int BS, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64, sc_waves(HEAD, WAVES)) scaled_context_kernel(const ScAttention a) {
+__global__ void __launch_bounds__(WAVES * 64, sc_waves(HEAD)) scaled_context_kernel(const ScAttention a) {
   using C = ScCode<E4M3>;
   constexpr int TILE = WAVES * kScRows;
   constexpr int KT = sc_stage(HEAD), NT = KT / 32, KS = HEAD / 16, DB = sc_padded(HEAD) / 32;
@@ -434,15 +434,18 @@ int sc_launch_context(const ScAttention& a, int num_seqs, hipStream_t stream) {
   return SW_OK;
 }
 
+// (eight waves are for heads of 80 to 128: sc_plan)
 template <bool E4M3, int BS, int WAVES>
 int sc_context_by_head(const ScAttention& a, int num_seqs, hipStream_t stream) {
+  if constexpr (WAVES == 4) {
+    if (a.head_size == 64) return sc_launch_context<E4M3, 64, BS, WAVES>(a, num_seqs, stream);
+    if (a.head_size == 256) return sc_launch_context<E4M3, 256, BS, WAVES>(a, num_seqs, stream);
+  }
   switch (a.head_size) {
-    case 64: return sc_launch_context<E4M3, 64, BS, WAVES>(a, num_seqs, stream);
     case 80: return sc_launch_context<E4M3, 80, BS, WAVES>(a, num_seqs, stream);
     case 96: return sc_launch_context<E4M3, 96, BS, WAVES>(a, num_seqs, stream);
     case 112: return sc_launch_context<E4M3, 112, BS, WAVES>(a, num_seqs, stream);
-    case 128: return sc_launch_context<E4M3, 128, BS, WAVES>(a, num_seqs, stream);
-    default: return sc_launch_context<E4M3, 256, BS, WAVES>(a, num_seqs, stream);
+    default: return sc_launch_context<E4M3, 128, BS, WAVES>(a, num_seqs, stream);
   }
 }
 
