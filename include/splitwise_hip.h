@@ -57,8 +57,9 @@ const char* sw_last_error(void);
  * 8: sw_prefill_attention_and_cache added.
  * 9: sw_paged_attention_and_cache added.
  * 10: sw_reshape_and_cache_scaled, sw_gather_cache_scaled, sw_paged_attention_scaled, sw_context_attention_scaled,
- *     sw_scaled_attention_parts, sw_scaled_attention_workspace_bytes added. */
-#define SW_ABI_VERSION 10
+ *     sw_scaled_attention_parts, sw_scaled_attention_workspace_bytes added.
+ * 11: sw_reshape_and_cache_scaled_indexed, sw_reshape_and_cache_scaled_indexed_workspace_bytes added. */
+#define SW_ABI_VERSION 11
 int sw_abi_version(void);
 
 /* csrc/cuda_utils_kernels.cu:16-35 get_max_shared_memory_per_block_device_attribute:
@@ -433,12 +434,20 @@ int sw_context_attention_split(void* out, const void* query, const void* key, co
  * magnitudes below 2^-100 count as 0), code = x / scale to the nearest, infinities the largest code, NaN 0; codes that are there are
  * rescaled.  A token for a block's first slot starts the block over: what it held, scales too, goes, and its other slots are zeros
  * unless the call writes them.  Slots outside 0 .. num_blocks * block_size - 1 are padding.  Tokens of one block may stand anywhere
- * in the list.  Of several tokens for one slot the last one stays, unless one run of neighbours in the list fills the whole block
- * in order: then the block's codes and scales may be either's, or some of each. */
+ * in the list.  Of several tokens for one slot the last one stays. */
 int sw_reshape_and_cache_scaled(const void* key, const void* value, void* key_cache, void* value_cache,
                                 float* key_scales, float* value_scales, const int64_t* slot_mapping, int num_tokens,
                                 int num_heads, int head_size, int block_size, int64_t num_blocks, int64_t key_stride,
                                 int64_t value_stride, int act_dtype, int cache_dtype, void* stream);
+
+/* The same with a workspace (4-byte aligned, any contents; 0 bytes and NULL for short lists), in which a first kernel finds out whether
+ * each block has its tokens side by side in the list.  Where they have, blocks of a long list need no look at the rest of it. */
+int sw_reshape_and_cache_scaled_indexed(const void* key, const void* value, void* key_cache, void* value_cache,
+                                        float* key_scales, float* value_scales, const int64_t* slot_mapping,
+                                        int num_tokens, int num_heads, int head_size, int block_size,
+                                        int64_t num_blocks, int64_t key_stride, int64_t value_stride, int act_dtype,
+                                        int cache_dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t sw_reshape_and_cache_scaled_indexed_workspace_bytes(int num_tokens, int64_t num_blocks);
 
 /* Reads seq_lens[i] tokens of block_tables row i back into rows seq_starts[i] .. of key and value ([num_rows, num_heads,
  * head_size], SW_F32 / SW_F16 / SW_BF16, rows on 16 bytes): code * scale, rounded once.  Tokens from max_seq_len (rounded up to whole

@@ -223,3 +223,16 @@ def test_every_kernel_that_is_built_is_launched():
     built = {(int(e), int(head), int(block), int(waves)) for e, head, block, waves in names}
     assert built == {(e, head, block, waves) for e in (0, 1) for block in (8, 16, 32) for waves in (4, 8)
                      for head in ((64, 80, 96, 112, 128, 256) if waves == 4 else (80, 96, 112, 128))}
+
+
+def test_workspace_of_a_long_list():
+    """None for lists that are gone through; a number for each block and one more for others.  What is too small is refused."""
+    lib = _C.load_library()
+    size = lib.sw_reshape_and_cache_scaled_indexed_workspace_bytes
+    assert size(0, 6) == size(1, 6) == size(256, 1 << 20) == 0
+    assert size(5000, 6) == 28 and size(5000, (1 << 31) - 1) == 1 << 33
+    p = ctypes.c_void_p(1 << 20)
+    for work, nbytes in ((p, 24), (ctypes.c_void_p((1 << 20) + 2), 28)):
+        status = lib.sw_reshape_and_cache_scaled_indexed(p, p, p, p, p, p, p, 5000, 2, 64, 16, 6, 128, 128, _C.SW_F32, _C.SW_E4M3_SCALED, work,
+                                                         nbytes, None)
+        assert status == -1 and "workspace" in lib.sw_last_error().decode()

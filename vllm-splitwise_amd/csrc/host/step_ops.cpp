@@ -28,8 +28,9 @@ namespace {
   X(swm_gated_delta_chunked) X(swm_gated_delta_chunked_workspace_floats) X(swm_head_norm_gate_act) X(swm_group_pairs)   \
   X(swm_expert_up_weighted) X(swm_expert_down_weighted) X(swm_masked_attention) X(swm_sink_attention)                   \
   X(swm_masked_attention_workspace_floats) X(swm_gla) X(swm_gla_workspace_floats) X(swm_lightning) X(swm_retention)     \
-  X(swm_lightning_workspace_floats) X(sw_reshape_and_cache_scaled) X(sw_gather_cache_scaled) X(sw_paged_attention_scaled)  \
-  X(sw_context_attention_scaled) X(sw_scaled_attention_parts) X(sw_scaled_attention_workspace_bytes)
+  X(swm_lightning_workspace_floats) X(sw_reshape_and_cache_scaled_indexed) X(sw_gather_cache_scaled) X(sw_paged_attention_scaled)  \
+  X(sw_context_attention_scaled) X(sw_scaled_attention_parts) X(sw_scaled_attention_workspace_bytes)                      \
+  X(sw_reshape_and_cache_scaled_indexed_workspace_bytes)
 // entry points of the libraries, set by bind() when one is loaded
 #define DECLARE(name) decltype(&::name) name##_at = nullptr;
 STEP_OPS(DECLARE)
@@ -358,18 +359,22 @@ void scaled_table(const Tensor& tables, std::initializer_list<const Tensor*> len
 STEP_OP(reshape_and_cache_scaled) {
   return call([&] {
     const Args c(args, nargs, 8);
-    take(sw_reshape_and_cache_scaled_at != nullptr);
+    take(sw_reshape_and_cache_scaled_indexed_at != nullptr);
     const Tensor &key = c.tensor(0), &value = c.tensor(1), &slots = c.tensor(6);
     const ScaledCache k(c, 2, args[7]);
     scaled_rows(key, value);
     const int act = hip_act(key);
     take(key.size(1) == k.heads && key.size(2) == k.size && slots.scalar_type() == at::kLong && slots.dim() == 1
          && slots.size(0) == key.size(0) && slots.is_contiguous());
+    const int64_t need = sw_reshape_and_cache_scaled_indexed_workspace_bytes_at((int)key.size(0), k.blocks);
+    const Tensor work = need > 0 ? at::empty({need}, key.options().dtype(at::kByte)) : Tensor();
+    void* scratch = need > 0 ? ptr<void>(work) : nullptr;
     void* stream = c.stream();
     return PyLong_FromLong(unlocked([&] {
-      return sw_reshape_and_cache_scaled_at(ptr<void>(key), ptr<void>(value), ptr<void>(k.key), ptr<void>(k.value), ptr(k.key_scales),
-                                            ptr(k.value_scales), ptr<int64_t>(slots), (int)key.size(0), (int)k.heads, (int)k.size,
-                                            k.block, k.blocks, key.stride(0), value.stride(0), act, k.type, stream);
+      return sw_reshape_and_cache_scaled_indexed_at(ptr<void>(key), ptr<void>(value), ptr<void>(k.key), ptr<void>(k.value),
+                                                    ptr(k.key_scales), ptr(k.value_scales), ptr<int64_t>(slots), (int)key.size(0),
+                                                    (int)k.heads, (int)k.size, k.block, k.blocks, key.stride(0), value.stride(0), act,
+                                                    k.type, scratch, need, stream);
     }));
   });
 }

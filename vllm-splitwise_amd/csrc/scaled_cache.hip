@@ -8,9 +8,10 @@
 //
 // One workgroup does all tokens of a block for two heads, a wave each for K and V of a head, because the scale is one for all of
 // them and what was there has to be read, rescaled and written by the same hands.  The slots' list has no order that one could rely
-// on.  A workgroup looks at `window` entries of it; those whose predecessor is in another block are heads of runs.  A run that
-// covers its whole block in order needs no look at the rest of the list; for any other one the workgroup goes through the whole list,
-// leaves if an earlier entry has the same block, and otherwise gathers the entries of that block, wherever they stand.
+// on, and may name blocks and slots more than once.  A workgroup looks at `window` entries of it; those whose predecessor is in another
+// block are heads of runs.  For a run's head the workgroup goes through the whole list, leaves if an earlier entry has the same block, and
+// otherwise gathers the entries of that block, wherever they stand.  In a long list that costs more than the blocks, and is for nothing
+// where each block has one run, as in a list of whole sequences: so where there is a workspace, two small launches find that out first.
 #include "scaled_cache.cuh"
 
 #include <algorithm>
@@ -26,6 +27,7 @@ struct ScWrite {
   const int64_t* slots;
   int64_t stride[2];           // elements from token to token
   int64_t num_slots;           // blocks * block size
+  const int* repeated;         // 0: no block has two runs, and no run more entries than its block slots; null: not known
   int num_tokens, heads, head_size, window, head_pairs;
 };
 
@@ -111,12 +113,17 @@ __device__ __forceinline__ uint32_t sc_rescale(uint32_t w, float ratio) {
 
 constexpr int kScWindow = 16;        // entries of a workgroup; they, one before them and a block behind them are a wave's lanes
 constexpr int kScLook = 16;          // entries that a thread asks for at a time as it goes through the list
+// Entries of a list that is gone through for each of its runs.  (us, gone through / looked at first, in two launches: 2444 tokens of 32 heads
+// 17.7 / 17.6, 3840 of 8 heads 11.6 / 11.7, 14293 44.5 / 22.4, 60000 443 / 78.)
+constexpr int kScShort = 1024;
 
 // Bound by vector instructions as much as by memory (an element is 2 bytes in and 1 out), so: a lane's addresses are one number and what
 // the compiler can put into the instructions; magnitudes two at a time; codes of finite values, the rule, in 4 instructions an element; and
-// blocks that the call fills look at no single token.  5 prompts of some 400 tokens, 32 heads of 128, f16 to e4m3 15.6 us, 16384 tokens of 8 heads
-// in whole blocks 22 us, 4.5 TB/s; 64 single tokens of 32 heads 6.7 us, of which the kernel's own chain of loads (list, list, token) is most.
-// Asking for a short list and for what a block holds earlier made the chain shorter and the rest slower: 0.1 us more there, 1 us more for prompts.
+// blocks that the call fills look at no single token.  5 prompts of some 400 tokens, 32 heads of 128, f16 to e4m3 17.6 us, 16384 tokens of 8 heads
+// in whole blocks 23 us, 4.4 TB/s, of which the look at the list is 3.5; 64 single tokens of 32 heads 6.5 us, of which the kernel's own chain of
+// loads (list, list, token) is most.  (Asking for a short list and for what a block holds earlier made the chain shorter and the rest slower:
+// 0.1 us more there, 1 us more for prompts.  The look at a long list in one launch of one workgroup: 16 us more for 16384 entries; at every
+// block_size-th entry by each workgroup of a run that fills its block, the other runs in a launch of their own: 11 us more.)
 
 // A lane's pieces are 16 elements of the key of one token, the same for all its pieces: 32 bytes in (64 of fp32), 16 out, where a wave's lie
 // side by side.  FULL: tokens first, first + 1, ... fill the block.
@@ -278,46 +285,72 @@ __device__ __forceinline__ void sc_write_values(const ScWrite& w, int64_t block,
   }
 }
 
+__device__ __forceinline__ int64_t sc_slot(const ScWrite& w, int64_t t) { return t >= 0 && t < w.num_tokens ? w.slots[t] : -1; }
+template <int BS>
+__device__ __forceinline__ int64_t sc_block(const ScWrite& w, int64_t slot) { return slot >= 0 && slot < w.num_slots ? slot / BS : -1; }
+
+// Whether the list names blocks in more than one run, or in one of more than BS entries, in two launches.  The heads of all runs enter
+// themselves in `owner` (an entry for each block, whose contents before do not matter); then each looks whether it is still there.
+template <int BS, bool ENTER>
+__global__ void __launch_bounds__(256) scaled_index_kernel(const ScWrite w, int* owner, int* repeated) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t block = sc_block<BS>(w, sc_slot(w, i)), before = sc_block<BS>(w, sc_slot(w, i - 1));
+  const bool head = block >= 0 && block != before;
+  if constexpr (ENTER) {
+    if (i == 0) *repeated = 0;
+    if (head) owner[block] = (int)i;
+  } else {
+    if ((head && owner[block] != (int)i) || (block >= 0 && sc_block<BS>(w, sc_slot(w, i - BS)) == block)) *repeated = 1;
+  }
+}
+
 template <typename act_t, bool E4M3, int BS, int DMAX>
 __global__ void __launch_bounds__(256) scaled_write_kernel(const ScWrite w) {
-  __shared__ int map[BS], earlier;
+  __shared__ int map[BS], leave, more;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // (all heads of a stretch of the list side by side in time: a token's row, and a block, are whole then)
   const int stretch = blockIdx.x / w.head_pairs, head = (blockIdx.x - stretch * w.head_pairs) * 2 + (wave >> 1);
   const int t0 = stretch * w.window;
-  auto block_of = [&](int64_t slot) -> int64_t { return slot >= 0 && slot < w.num_slots ? slot / BS : -1; };
-  auto slot_of = [&](int t) -> int64_t { return t >= 0 && t < w.num_tokens ? w.slots[t] : -1; };
 
   // lane l: entry t0 - 1 + l (its block), of which `window` are this workgroup's; those whose predecessor is in another block are heads
   // of runs (every wave finds the same ones)
-  const int64_t near = slot_of(t0 - 1 + lane), near_block = block_of(near), before = __shfl_up(near_block, 1, 64);
+  const int64_t near = sc_slot(w, t0 - 1 + lane), near_block = sc_block<BS>(w, near), before = __shfl_up(near_block, 1, 64);
+  const bool alone = w.repeated != nullptr && *w.repeated == 0;
   uint64_t heads = __ballot(lane >= 1 && lane <= w.window && near_block >= 0 && near_block != before);
   while (heads) {
     const int at = __builtin_ctzll(heads), t = t0 - 1 + at;
     heads &= heads - 1;
     const int64_t first = __shfl(near, at, 64), block = first / BS;
-    // the whole block in order, and nothing of it right behind (a window and a block behind it are lanes of the wave)
-    const bool as_run = lane < at || lane > at + BS || (lane < at + BS ? near == first + (lane - at) : near_block != block);
-    const bool full = first % BS == 0 && __ballot(as_run) == ~0ull;
-    if (!full) {
-      __syncthreads();                                          // the last run's map has been read
+    // the run, and whether it is the whole block in order (a window and a block behind it are lanes of the wave)
+    const uint64_t others = ~(__ballot(near_block == block) >> at);
+    const int entries = others ? __builtin_ctzll(others) : 64;
+    const bool in_order = lane < at || lane >= at + BS || near == first + (lane - at);
+    bool full = first % BS == 0 && entries == BS && __ballot(in_order) == ~0ull;
+    if (!(alone && full)) {
+      __syncthreads();                                          // the last run's map and flags have been read
       if (threadIdx.x < BS) map[threadIdx.x] = -1;
-      if (threadIdx.x == BS) earlier = 0;
+      if (threadIdx.x == BS) leave = more = 0;
       __syncthreads();
-      for (int i0 = threadIdx.x; i0 < w.num_tokens; i0 += 256 * kScLook) {
-        int64_t s[kScLook];
+      if (alone) {
+        if (wave == 0 && lane >= at && lane < at + entries) atomicMax(&map[near % BS], t0 - 1 + lane);
+      } else {
+        for (int i0 = threadIdx.x; i0 < w.num_tokens; i0 += 256 * kScLook) {
+          int64_t s[kScLook];
 #pragma unroll
-        for (int k = 0; k < kScLook; ++k) s[k] = slot_of(i0 + 256 * k);
+          for (int k = 0; k < kScLook; ++k) s[k] = sc_slot(w, i0 + 256 * k);
 #pragma unroll
-        for (int k = 0; k < kScLook; ++k) {
-          const int i = i0 + 256 * k;
-          if (block_of(s[k]) != block) continue;
-          if (i < t) earlier = 1;
-          else atomicMax(&map[s[k] % BS], i);                   // of two tokens for one slot the later one
+          for (int k = 0; k < kScLook; ++k) {
+            const int i = i0 + 256 * k;
+            if (sc_block<BS>(w, s[k]) != block) continue;
+            if (i < t) leave = 1;
+            else atomicMax(&map[s[k] % BS], i);                 // of two tokens for one slot the later one
+            if (i >= t + BS) more = 1;
+          }
         }
       }
       __syncthreads();
-      if (earlier) continue;                                    // that entry's workgroup does the block
+      if (leave) continue;                                      // that entry's workgroup does the block
+      full = full && !more;
     }
     if (head >= w.heads) continue;
     if (full) {
@@ -470,10 +503,14 @@ bool sc_aligned(const void* p, int64_t stride, int size) { return (uintptr_t)p %
 
 extern "C" {
 
-int sw_reshape_and_cache_scaled(const void* key, const void* value, void* key_cache, void* value_cache, float* key_scales,
-                                float* value_scales, const int64_t* slot_mapping, int num_tokens, int num_heads, int head_size,
-                                int block_size, int64_t num_blocks, int64_t key_stride, int64_t value_stride, int act_dtype,
-                                int cache_dtype, void* stream) {
+int64_t sw_reshape_and_cache_scaled_indexed_workspace_bytes(int num_tokens, int64_t num_blocks) {
+  return num_tokens <= sw::kScShort || num_blocks <= 0 ? 0 : (num_blocks + 1) * 4;
+}
+
+int sw_reshape_and_cache_scaled_indexed(const void* key, const void* value, void* key_cache, void* value_cache, float* key_scales,
+                                        float* value_scales, const int64_t* slot_mapping, int num_tokens, int num_heads, int head_size,
+                                        int block_size, int64_t num_blocks, int64_t key_stride, int64_t value_stride, int act_dtype,
+                                        int cache_dtype, void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace sw;
   const int bad = sc_check("reshape_and_cache_scaled", num_heads, head_size, block_size, num_blocks, act_dtype, cache_dtype);
   if (bad) return bad;
@@ -482,6 +519,9 @@ int sw_reshape_and_cache_scaled(const void* key, const void* value, void* key_ca
   SW_CHECK_ARG(sc_aligned(key, key_stride, es) && sc_aligned(value, value_stride, es) && (uintptr_t)key_cache % 16 == 0 &&
                    (uintptr_t)value_cache % 16 == 0,
                "reshape_and_cache_scaled: rows of keys and values, and the caches, must begin on multiples of 16 bytes");
+  SW_CHECK_ARG(workspace == nullptr || ((uintptr_t)workspace % 4 == 0 &&
+                                        workspace_bytes >= sw_reshape_and_cache_scaled_indexed_workspace_bytes(num_tokens, num_blocks)),
+               "reshape_and_cache_scaled: the workspace for %d tokens is too small or not aligned", num_tokens);
   if (num_tokens == 0) return SW_OK;
   ScWrite w;
   w.x[0] = key, w.x[1] = value;
@@ -493,10 +533,24 @@ int sw_reshape_and_cache_scaled(const void* key, const void* value, void* key_ca
   w.num_tokens = num_tokens, w.heads = num_heads, w.head_size = head_size;
   // a decode step's entries each begin a run, a prompt's only every block_size-th
   static_assert(1 + kScWindow + 32 <= 64, "");
-  w.window = num_tokens <= 1024 ? 1 : kScWindow;
+  w.window = num_tokens <= kScShort ? 1 : kScWindow;
   w.head_pairs = (num_heads + 1) / 2;
   const int64_t workgroups = ((int64_t)num_tokens + w.window - 1) / w.window * w.head_pairs;
   SW_CHECK_ARG(workgroups <= kScMostWorkgroups, "reshape_and_cache_scaled: %d tokens of %d heads are too many for a call", num_tokens, num_heads);
+  w.repeated = nullptr;
+  if (workspace && num_tokens > kScShort) {
+    int* const repeated = (int*)workspace;
+    w.repeated = repeated;
+    auto index = [&](auto bs) {
+      const unsigned groups = ((unsigned)num_tokens + 255) / 256;
+      scaled_index_kernel<decltype(bs)::value, true><<<groups, 256, 0, (hipStream_t)stream>>>(w, repeated + 1, repeated);
+      scaled_index_kernel<decltype(bs)::value, false><<<groups, 256, 0, (hipStream_t)stream>>>(w, repeated + 1, repeated);
+    };
+    block_size == 8    ? index(std::integral_constant<int, 8>{})
+    : block_size == 16 ? index(std::integral_constant<int, 16>{})
+                       : index(std::integral_constant<int, 32>{});
+    SW_CHECK_LAUNCH();
+  }
   const dim3 grid((unsigned)workgroups);
   return sc_by_type(act_dtype, cache_dtype, [&](auto a, auto e) {
     return sc_by_size(head_size, block_size, [&](auto bs, auto d) -> int {
@@ -506,6 +560,15 @@ int sw_reshape_and_cache_scaled(const void* key, const void* value, void* key_ca
       return SW_OK;
     });
   });
+}
+
+int sw_reshape_and_cache_scaled(const void* key, const void* value, void* key_cache, void* value_cache, float* key_scales,
+                                float* value_scales, const int64_t* slot_mapping, int num_tokens, int num_heads, int head_size,
+                                int block_size, int64_t num_blocks, int64_t key_stride, int64_t value_stride, int act_dtype,
+                                int cache_dtype, void* stream) {
+  return sw_reshape_and_cache_scaled_indexed(key, value, key_cache, value_cache, key_scales, value_scales, slot_mapping, num_tokens,
+                                             num_heads, head_size, block_size, num_blocks, key_stride, value_stride, act_dtype, cache_dtype,
+                                             nullptr, 0, stream);
 }
 
 int sw_gather_cache_scaled(void* key, void* value, const void* key_cache, const void* value_cache, const float* key_scales,

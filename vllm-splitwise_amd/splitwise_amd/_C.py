@@ -82,6 +82,8 @@ _SIGNATURES = {
     "sw_context_attention_split_parts": [_c_int] * 6,
     "sw_context_attention_split_workspace_bytes": [_c_int, _c_i64, _c_int, _c_int],
     "sw_reshape_and_cache_scaled": [_c_void_p] * 7 + [_c_int] * 4 + [_c_i64] * 3 + [_c_int] * 2 + [_c_void_p],
+    "sw_reshape_and_cache_scaled_indexed": [_c_void_p] * 7 + [_c_int] * 4 + [_c_i64] * 3 + [_c_int] * 2 + [_c_void_p, _c_i64, _c_void_p],
+    "sw_reshape_and_cache_scaled_indexed_workspace_bytes": [_c_int, _c_i64],
     "sw_gather_cache_scaled": [_c_void_p] * 9 + [_c_int] * 2 + [_c_i64] + [_c_int] * 3 + [_c_i64, _c_int] + [_c_i64] * 3
                               + [_c_int] * 2 + [_c_void_p],
     "sw_paged_attention_scaled": [_c_void_p] * 6 + [_c_int] * 4 + [_c_float] + [_c_void_p] * 2 + [_c_int, _c_i64, _c_int, _c_int, _c_i64]
@@ -113,7 +115,8 @@ _SIGNATURES = {
 _RESTYPES = {"sw_quant_gemm_workspace_bytes": _c_i64, "sw_custom_ar_signal_bytes": _c_i64,
              "sw_paged_attention_v2_static_max_bytes": _c_i64,
              "sw_context_attention_split_workspace_bytes": _c_i64,
-             "sw_scaled_attention_workspace_bytes": _c_i64}     # everything else returns an int status
+             "sw_scaled_attention_workspace_bytes": _c_i64,
+             "sw_reshape_and_cache_scaled_indexed_workspace_bytes": _c_i64}     # everything else returns an int status
 
 _lib = None
 
@@ -122,7 +125,7 @@ def library_path() -> str:
     return _LIB_PATH
 
 
-ABI_VERSION = 10               # SW_ABI_VERSION of include/splitwise_hip.h this binding was written against
+ABI_VERSION = 11               # SW_ABI_VERSION of include/splitwise_hip.h this binding was written against
 
 
 def load_library() -> ctypes.CDLL:
@@ -626,8 +629,7 @@ def reshape_and_cache_scaled(key: torch.Tensor, value: torch.Tensor, key_cache: 
     A block's scale is its largest finite magnitude over 127 (448).  It grows when a call brings a larger one, and what the block held
     is rescaled; it starts over with the token for the block's first slot, whose other slots become zeros unless the call writes them.
     Infinities go to the largest code, NaN to 0.  Slots outside the cache (negative: padding) are skipped.  A block's
-    tokens may stand anywhere in the list, and of several for one slot the last one stays (unless neighbours in the list fill the whole
-    block in order: then the block may hold either's codes and scale, or some of each)."""
+    tokens may stand anywhere in the list, and of several for one slot the last one stays."""
     status = _native.reshape_and_cache_scaled(key, value, key_cache, value_cache, key_scales, value_scales, slot_mapping, kv_cache_dtype)
     if status is not None:
         return _check(status)
@@ -637,11 +639,16 @@ def reshape_and_cache_scaled(key: torch.Tensor, value: torch.Tensor, key_cache: 
         raise RuntimeError(f"{name}: slot_mapping must be contiguous int64, one for each token")
     cache = _scaled_caches(name, kv_cache_dtype, key, key.shape[2], key.shape[1], key_cache, value_cache, key_scales, value_scales,
                            value, slot_mapping)
+    lib = load_library()
     with _on_device_of(key):
-        _check(load_library().sw_reshape_and_cache_scaled(
+        # (from torch's caching allocator, so that a captured call has its own)
+        nbytes = int(lib.sw_reshape_and_cache_scaled_indexed_workspace_bytes(key.shape[0], value_cache.shape[0]))
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=key.device) if nbytes else None
+        _check(lib.sw_reshape_and_cache_scaled_indexed(
             key.data_ptr(), value.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(), key_scales.data_ptr(),
             value_scales.data_ptr(), slot_mapping.data_ptr(), key.shape[0], key.shape[1], key.shape[2], value_cache.shape[3],
-            value_cache.shape[0], key.stride(0), value.stride(0), _act_dtype(key), cache, _stream(key)))
+            value_cache.shape[0], key.stride(0), value.stride(0), _act_dtype(key), cache, workspace.data_ptr() if nbytes else None, nbytes,
+            _stream(key)))
 
 
 def gather_cache_scaled(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
