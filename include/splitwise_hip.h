@@ -86,7 +86,8 @@ int sw_reshape_and_cache(const void* key, const void* value, void* key_cache,
  * block dst[p] of key_cache_ptrs[l] and of value_cache_ptrs[l] := block src[p].
  *   key_cache_ptrs / value_cache_ptrs  DEVICE arrays of num_layers device pointers
  *   block_mapping                      DEVICE int64 [num_pairs][2] = (src, dst)
- *   block_bytes                        bytes of one block of one tensor, multiple of 16 */
+ *   block_bytes                        bytes of one block of one tensor: a multiple of 16, with tensors that begin
+ *                                      on 16 bytes, or one of 4, with tensors that begin on 4 */
 int sw_copy_blocks(const void* const* key_cache_ptrs,
                    const void* const* value_cache_ptrs, int num_layers,
                    const int64_t* block_mapping, int num_pairs,

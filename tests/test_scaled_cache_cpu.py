@@ -236,3 +236,10 @@ def test_workspace_of_a_long_list():
         status = lib.sw_reshape_and_cache_scaled_indexed(p, p, p, p, p, p, p, 5000, 2, 64, 16, 6, 128, 128, _C.SW_F32, _C.SW_E4M3_SCALED, work,
                                                          nbytes, None)
         assert status == -1 and "workspace" in lib.sw_last_error().decode()
+
+
+def test_blocks_of_odd_bytes_are_not_copied():
+    lib = _C.load_library()
+    p = ctypes.c_void_p(1 << 20)
+    for nbytes in (2, 6, 17, 0, -4):
+        assert lib.sw_copy_blocks(p, p, 1, p, 1, nbytes, None) == -1 and "block_bytes" in lib.sw_last_error().decode()

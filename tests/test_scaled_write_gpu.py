@@ -145,3 +145,16 @@ def test_long_lists_in_graphs_that_share_their_memory(kind):
         for i in range(2):
             run(twins[i], i)
             assert all(torch.equal(a, b) for a, b in zip(caches[i].device, twins[i].device))
+
+
+@pytest.mark.parametrize("heads", [1, 2, 3, 4, 5, 8, 40])
+@pytest.mark.parametrize("offset", [0, 1, 2])
+def test_scales_of_any_number_of_heads_are_copied(heads, offset):
+    """A block's scales are 4 bytes a head: blocks of no multiple of 16 bytes begin on 4; those of other blocks stay."""
+    from splitwise_amd import _C
+    offset = 4 * offset if heads % 4 == 0 else offset
+    some = [torch.rand(7 * heads + offset, device=DEV)[offset:].view(7, heads) for _ in range(6)]
+    before = [t.clone() for t in some]
+    _C.cache_ops.copy_blocks(some[:3], some[3:], {1: [2, 3], 5: [6]})
+    for now, was in zip(some, before):
+        assert torch.equal(now, was[[0, 1, 1, 1, 4, 5, 5]])

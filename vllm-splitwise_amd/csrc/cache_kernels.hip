@@ -10,7 +10,7 @@
 //     With consecutive slots (a prompt) one wave store covers contiguous
 //     256-byte (K) / 1-KiB (V) pieces of the 4-KiB [block, head] cache tile; with
 //     arbitrary slots (decode) every token is still placed individually.
-//   * copy_blocks moves 16 bytes per lane with the pointer tables resident on
+//   * copy_blocks moves 16 bytes per lane (4 where blocks are no multiple of 16) with the pointer tables resident on
 //     the device (no per-call pointer upload).
 #include "cache_tile.cuh"
 
@@ -39,7 +39,9 @@ __global__ void __launch_bounds__(kRcThreads) reshape_and_cache_tile_kernel(cons
   cache_tile<act_t, FP8, VT>(w, blockIdx.x, threadIdx.x, smem);
 }
 
-// Grid: (2 * num_pairs, num_layers, splits).  blockIdx.x even = K, odd = V.
+// Grid: (2 * num_pairs, num_layers, splits).  blockIdx.x even = K, odd = V.  Vec: 16 bytes, or 4 for blocks of another size (the scales of
+// a block of an 8-bit cache).
+template <typename Vec>
 __global__ void __launch_bounds__(256)
 copy_blocks_kernel(const void* const* __restrict__ key_ptrs,
                    const void* const* __restrict__ value_ptrs,
@@ -47,11 +49,11 @@ copy_blocks_kernel(const void* const* __restrict__ key_ptrs,
   const int pair = blockIdx.x >> 1;
   const bool is_v = blockIdx.x & 1;
   const int layer = blockIdx.y;
-  uint4* base = reinterpret_cast<uint4*>(const_cast<void*>(is_v ? value_ptrs[layer] : key_ptrs[layer]));
+  Vec* base = reinterpret_cast<Vec*>(const_cast<void*>(is_v ? value_ptrs[layer] : key_ptrs[layer]));
   const int64_t src = mapping[2 * pair];
   const int64_t dst = mapping[2 * pair + 1];
-  const uint4* s = base + src * vecs_per_block;
-  uint4* d = base + dst * vecs_per_block;
+  const Vec* s = base + src * vecs_per_block;
+  Vec* d = base + dst * vecs_per_block;
   for (int64_t i = (int64_t)blockIdx.z * blockDim.x + threadIdx.x; i < vecs_per_block;
        i += (int64_t)gridDim.z * blockDim.x) {
     d[i] = s[i];
@@ -194,14 +196,15 @@ int sw_copy_blocks(const void* const* key_cache_ptrs, const void* const* value_c
                    int64_t block_bytes, void* stream) {
   using namespace sw;
   if (num_layers == 0 || num_pairs == 0) return SW_OK;
-  SW_CHECK_ARG(num_layers > 0 && num_pairs > 0 && block_bytes > 0 && block_bytes % 16 == 0,
+  SW_CHECK_ARG(num_layers > 0 && num_pairs > 0 && block_bytes > 0 && block_bytes % 4 == 0,
                "copy_blocks: bad arguments (layers=%d pairs=%d block_bytes=%lld)", num_layers,
                num_pairs, (long long)block_bytes);
   SW_CHECK_ARG(num_layers <= 65535, "copy_blocks: too many layers");
-  const int64_t vecs = block_bytes / 16;
+  const bool wide = block_bytes % 16 == 0;
+  const int64_t vecs = block_bytes / (wide ? 16 : 4);
   const int splits = (int)std::min<int64_t>(32, std::max<int64_t>(1, vecs / 1024));
   dim3 grid(2 * num_pairs, num_layers, splits);
-  copy_blocks_kernel<<<grid, 256, 0, static_cast<hipStream_t>(stream)>>>(
+  (wide ? copy_blocks_kernel<uint4> : copy_blocks_kernel<uint32_t>)<<<grid, 256, 0, static_cast<hipStream_t>(stream)>>>(
       key_cache_ptrs, value_cache_ptrs, block_mapping, vecs);
   SW_CHECK_LAUNCH();
   return SW_OK;

@@ -128,10 +128,9 @@ class CacheEngine:
     def copy(self, src_to_dsts: Dict[int, List[int]]) -> None:
         # one launch for all layers; runs on the compute stream, so it is ordered before the step
         _C.cache_ops.copy_blocks([k for k, _ in self.gpu_cache], [v for _, v in self.gpu_cache], src_to_dsts)
-        pairs = [(src, dst) for src, dsts in src_to_dsts.items() for dst in dsts]
-        if self.gpu_scales is not None and pairs:
-            src, dst = torch.tensor(pairs).to(self.gpu_scales.device).unbind(1)
-            self.gpu_scales[:, :, dst] = self.gpu_scales[:, :, src]
+        if self.gpu_scales is not None:
+            scales = [k.scales for k, _ in self.gpu_cache]
+            _C.cache_ops.copy_blocks([k for k, _ in scales], [v for _, v in scales], src_to_dsts)
 
     @staticmethod
     def get_cache_block_size(block_size: int, cache_dtype: str, model_config: ModelConfig,
