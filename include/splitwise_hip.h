@@ -433,7 +433,7 @@ int sw_context_attention_split(void* out, const void* query, const void* key, co
 /* Quantises [num_tokens, num_heads, head_size] keys and values (SW_F32 / SW_F16 / SW_BF16, rows on 16 bytes) into the
  * slots.  For the tokens of a call that go to one (block, head): scale = max(the block's, max |x| / 127 or / 448 over finite x;
  * magnitudes below 2^-100 count as 0), code = x / scale to the nearest, infinities the largest code, NaN 0; codes that are there are
- * rescaled.  A token for a block's first slot starts the block over: what it held, scales too, goes, and its other slots are zeros
+ * rescaled (those of a scale below 2^-110, which no call leaves, are zeros).  A token for a block's first slot starts the block over: what it held, scales too, goes, and its other slots are zeros
  * unless the call writes them.  Slots outside 0 .. num_blocks * block_size - 1 are padding.  Tokens of one block may stand anywhere
  * in the list.  Of several tokens for one slot the last one stays. */
 int sw_reshape_and_cache_scaled(const void* key, const void* value, void* key_cache, void* value_cache,

@@ -158,3 +158,25 @@ def test_scales_of_any_number_of_heads_are_copied(heads, offset):
     _C.cache_ops.copy_blocks(some[:3], some[3:], {1: [2, 3], 5: [6]})
     for now, was in zip(some, before):
         assert torch.equal(now, was[[0, 1, 1, 1, 4, 5, 5]])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("scale", [1e-45, 1e-39, 2.0 ** -127, 2.0 ** -111])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_a_scale_that_no_write_leaves_is_none(kind, scale, dtype):
+    """Zeros, and then numbers, for a block that was never written and whose memory holds a scale without a finite reciprocal."""
+    from oracle import scaled_cache as oracle
+    from splitwise_amd import _C
+    c = Cache(3, 2, 64, 16, kind)
+    c.ks.fill_(scale), c.vs.fill_(scale)
+    x = torch.zeros(1, 2, 64, dtype=dtype, device=DEV)
+    slot = torch.tensor([16 + 3], device=DEV)
+    _C.cache_ops.reshape_and_cache_scaled(x, x, *c.device, slot, kind)
+    for cache, scales in ((c.key, c.ks), (c.value, c.vs)):
+        assert (oracle.codes_of(cache.cpu(), kind)[1] == 0).all() and (scales[1] == 0).all()
+    x = torch.randn(1, 2, 64, generator=torch.Generator().manual_seed(1)).to(dtype).to(DEV)
+    _C.cache_ops.reshape_and_cache_scaled(x, x, *c.device, slot, kind)
+    for cache, scales in ((c.key, c.ks), (c.value, c.vs)):
+        got = oracle.codes_of(cache.cpu(), kind)[1] * scales.cpu()[1].double()[:, None]
+        assert (got[torch.arange(16) != 3] == 0).all()
+        assert (got[3] - x[0].cpu().double()).abs().max() <= float(x.abs().max()) * (0.51 / 127 if kind == "int8" else 2.0 ** -4)

@@ -71,8 +71,8 @@ __device__ __forceinline__ int sc_part_end(const ScAttention& a, const ScSequenc
   return part == a.parts - 1 ? end : min(end, (part + 1) * a.part_tokens);
 }
 
-// A value scale as a power of two.  Below 2^-110 it is that of a block of zeros: further down than any sum reaches.
-constexpr float kScLeast = 0x1p-110f, kScNone = -300.f;
+// A value scale as a power of two.  Less than any write leaves is that of a block of zeros: further down than any sum reaches.
+constexpr float kScNone = -300.f;
 __device__ __forceinline__ float sc_log_scale(float s) {
   return s < kScLeast ? kScNone : __builtin_amdgcn_logf(s);  // (a NaN stays one)
 }

@@ -103,8 +103,10 @@ template <> struct ScCode<true> {
   }
 };
 
-// A scale as an earlier write left it; a block that was never written may hold anything.
-__device__ __forceinline__ float sc_old_scale(float s) { return s > 0.f && s < INFINITY ? s : 0.f; }
+// A scale as an earlier write left it: 0, or at least kScTiny / 448.  A block that was never written may hold anything, also what has no
+// finite reciprocal.
+constexpr float kScLeast = 0x1p-110f;
+__device__ __forceinline__ float sc_old_scale(float s) { return s >= kScLeast && s < INFINITY ? s : 0.f; }
 
 inline bool sc_head_size(int d) { return d == 64 || d == 80 || d == 96 || d == 112 || d == 128 || d == 256; }
 
