@@ -246,3 +246,18 @@ def test_all_scales_far_from_one(kind, size, block, heads, kv_heads, power, part
         got = decode(c, query[:2], tables, lens, 0.09, parts=parts)
         check(got, c, query[:2], tables, lens, [1, 1], 0.09)
         c = Cache(len(c.value_scales), kv_heads, size, block, kind)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5, 2 ** 40, 48, 100000])
+@pytest.mark.parametrize("heads", [1, 8])
+def test_windows_wider_than_any_context(kind, window, heads):
+    """They hide nothing, also behind rows that stand before the sequence's first token."""
+    new, lens = [70, 3], [40, 48]
+    c = Cache(7, 1, 64, 16, kind)
+    tables = tables_for(lens, 16, 7)
+    query = random_query(73, heads, 64, torch.bfloat16)
+    got = context(c, query, tables, [0, 70], new, lens, 0.1, window=window)
+    assert torch.equal(got, context(c, query, tables, [0, 70], new, lens, 0.1))
+    assert (got[:30] == 0).all()
+    check(got, c, query, tables, lens, new, 0.1)

@@ -162,6 +162,8 @@ int sc_attend(const char* what, ScAttention a, int num_seqs, int64_t num_blocks,
   SW_CHECK_ARG(num_parts == 1 || (workspace && (uintptr_t)workspace % 16 == 0 &&
                                   workspace_bytes >= sw_scaled_attention_workspace_bytes(num_parts, a.num_rows, a.heads, a.head_size)),
                "%s: the workspace for %d parts is missing, too small or not aligned", what, num_parts);
+  // (a window of all that a table holds hides nothing, and positions less it stay within 32 bits)
+  if (a.window >= a.width * block_size) a.window = 0;
   a.group = a.heads / a.kv_heads;
   SW_CHECK_ARG((int64_t)max_new_len * a.group < INT32_MAX / 2, "%s: %d new tokens", what, max_new_len);
   const ScPlan plan = sc_plan(num_seqs, max_new_len, a.heads, a.kv_heads, a.head_size, max_context_len);

@@ -763,7 +763,7 @@ def context_attention_scaled(out: torch.Tensor, query: torch.Tensor, key_cache: 
             value_scales.data_ptr(), seq_lens.shape[0], rows, num_heads, num_kv_heads, head_size, float(scale),
             block_tables.data_ptr(), seq_starts.data_ptr(), new_lens.data_ptr(), seq_lens.data_ptr(), value_cache.shape[3],
             value_cache.shape[0], int(max_new_len), int(max_context_len), block_tables.shape[1], block_tables.stride(0),
-            alibi_slopes.data_ptr() if alibi_slopes is not None else None, int(sliding_window) if sliding_window else 0,
+            alibi_slopes.data_ptr() if alibi_slopes is not None else None, max(0, min(int(sliding_window or 0), 2 ** 31 - 1)),
             query.stride(0), out.stride(0), _act_dtype(query), cache, num_parts, workspace.data_ptr() if nbytes else None, nbytes,
             _stream(query)))
 
