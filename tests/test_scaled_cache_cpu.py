@@ -243,3 +243,12 @@ def test_blocks_of_odd_bytes_are_not_copied():
     p = ctypes.c_void_p(1 << 20)
     for nbytes in (2, 6, 17, 0, -4):
         assert lib.sw_copy_blocks(p, p, 1, p, 1, nbytes, None) == -1 and "block_bytes" in lib.sw_last_error().decode()
+
+
+def test_the_reason_of_a_refused_option_is_its_own():
+    """Only pools of several workers have a transport: the option that runs both sides on one worker is not refused for it."""
+    from splitwise_amd.engine.arg_utils import EngineArgs
+    with pytest.raises(NotImplementedError) as told:
+        EngineArgs(model="llama-tiny", kv_cache_dtype="int8", overlap_prompt_decode=True, pipeline_steps=True).create_engine_configs()
+    text = str(told.value)
+    assert "overlap_prompt_decode, whose two streams" in text and "sep_prompt_token, as the transport" in text

@@ -63,8 +63,9 @@ class EngineArgs:
                                    self.kv_cache_dtype, model_config.get_sliding_window(),
                                    self.enable_prefix_caching)
         if self.kv_cache_dtype in SCALED_CACHE_DTYPES and (self.sep_prompt_token or self.overlap_prompt_decode):
-            raise NotImplementedError(f"kv_cache_dtype {self.kv_cache_dtype!r} keeps scales beside the cache, which the transport between "
-                                      "prompt and token pools does not carry: it excludes sep_prompt_token and overlap_prompt_decode")
+            raise NotImplementedError(f"kv_cache_dtype {self.kv_cache_dtype!r} keeps scales beside the cache.  It excludes sep_prompt_token, "
+                                      "as the transport between prompt and token pools does not carry them, and overlap_prompt_decode, "
+                                      "whose two streams have not been tried with a write that rescales what a block holds")
         if self.overlap_prompt_decode:
             # the engine runs its split loop (a prompt side and a token side that run free of each other) over ONE
             # worker: executor/overlap_executor.py
