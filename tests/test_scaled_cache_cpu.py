@@ -252,3 +252,13 @@ def test_the_reason_of_a_refused_option_is_its_own():
         EngineArgs(model="llama-tiny", kv_cache_dtype="int8", overlap_prompt_decode=True, pipeline_steps=True).create_engine_configs()
     text = str(told.value)
     assert "overlap_prompt_decode, whose two streams" in text and "sep_prompt_token, as the transport" in text
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8_e4m3"])
+def test_models_of_32_bits_are_refused_before_they_are_loaded(kind):
+    from splitwise_amd.engine.arg_utils import EngineArgs
+    with pytest.raises(NotImplementedError, match="float16 and bfloat16"):
+        EngineArgs(model="llama-tiny", dtype="float32", kv_cache_dtype=kind).create_engine_configs()
+    for dtype in ("auto", "float16", "bfloat16"):
+        EngineArgs(model="llama-tiny", dtype=dtype, kv_cache_dtype=kind).create_engine_configs()
+    EngineArgs(model="llama-tiny", dtype="float32", kv_cache_dtype="fp8_e5m2").create_engine_configs()

@@ -5,6 +5,8 @@ import dataclasses
 from dataclasses import dataclass
 from typing import Optional, Tuple
 
+import torch
+
 from ..config import SCALED_CACHE_DTYPES, CacheConfig, DeviceConfig, ModelConfig, ParallelConfig, SchedulerConfig
 
 
@@ -66,6 +68,8 @@ class EngineArgs:
             raise NotImplementedError(f"kv_cache_dtype {self.kv_cache_dtype!r} keeps scales beside the cache.  It excludes sep_prompt_token, "
                                       "as the transport between prompt and token pools does not carry them, and overlap_prompt_decode, "
                                       "whose two streams have not been tried with a write that rescales what a block holds")
+        if self.kv_cache_dtype in SCALED_CACHE_DTYPES and model_config.dtype == torch.float32:
+            raise NotImplementedError(f"the attention over kv_cache_dtype {self.kv_cache_dtype!r} takes float16 and bfloat16 models")
         if self.overlap_prompt_decode:
             # the engine runs its split loop (a prompt side and a token side that run free of each other) over ONE
             # worker: executor/overlap_executor.py
