@@ -126,11 +126,11 @@ ScPlan sc_plan(int num_seqs, int max_new_len, int num_heads, int num_kv_heads, i
     p.waves = head_size <= 128 && w <= (max_context_len >= 4096 && rows <= 16 ? 1024 : 256) ? 8 : 4;
     p.parts = (int)std::min<int64_t>(max_context_len < 1024 ? 1 : ((int64_t)max_context_len + 255) / 256, 256 / w);
   } else {
-    // 256 rows where there are enough of them: half the widening a row (us, 128 / 256 rows: 2041 tokens of 8 heads behind 14003 1063 / 998,
-    // 8 x 1024 behind 1000 331 / 325, 6 x 301 78 / 80, 30 x 50 behind 10 33 / 37; heads of 64, 8 x 1024, 212 / 248).
-    // Fewer than the 512 that run at once: parts, for whose sums each row costs 2 x 4 bytes a dim and part; short ones up to 256 workgroups, which
+    // 256 rows where there are enough of them: half the widening a row (us, 128 / 256 rows: 2041 tokens of 8 heads behind 14003 1063 / 1002,
+    // 8 x 1024 behind 1000 331 / 324, 6 x 301 78 / 80, 30 x 50 behind 10 33 / 37; heads of 64, 8 x 1024, 212 / 248).
+    // Fewer than the 512 that run at once (256 of heads of 256): parts, for whose sums each row costs 2 x 4 bytes a dim and part; short ones up to 256 workgroups, which
     // have few rows, and long ones up to 512 (us by parts: 120 tokens of 8 heads behind 3000 1 78.5, 4 30.7, 16 25.0, 48 25.2; behind 800 1 32.6,
-    // 4 21.7, 12 21.5; 2 x 42 of 8 heads of 256 on 2 behind 2049 1 320, 3 125, 16 44, 32 41; 400 of 32 on 8 behind 12000 1 282, 4 120, 6 133, 12 142;
+    // 4 21.7, 12 21.5; 2 x 42 of 8 heads of 256 on 2 behind 2007 1 139, 3 59, 10 35, 32 31; 2 x 1000 of 4 behind 1500 1 175, 3 81, 4 101; 400 of 32 on 8 behind 12000 1 282, 4 120, 6 133, 12 142;
     // 500 of 32 behind 4000 1 110, 2 76, 4 67, 8 78; 512 of 64 on 8 behind 8000 1 198, 2 180, 4 185; 800 behind 600 1 51, 2 77; 1000 of 32 heads
     // behind 100 1 39, 2 51).
     const int64_t w = workgroups(128);

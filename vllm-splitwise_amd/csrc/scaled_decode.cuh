@@ -24,7 +24,7 @@
 // into the row's scale.
 //
 // Measured (heads of 128): 61 sequences of some 1090 tokens, 32 heads, e4m3, 544 MB, 106 us, 5.2 TB/s, what a large copy reads and
-// writes; 201 of some 2000, 64 heads on 8, int8, 820 MB, 170 us, 4.8 TB/s (of one length 5.4: the longest
+// writes (a reading stream reaches 6.2); 201 of some 2000, 64 heads on 8, int8, 820 MB, 170 us, 4.8 TB/s (of one length 5.4: the longest
 // sequences' workgroups run on alone); 3 of 34000 to 90000, 64 on 8, e4m3 in ten parts and their join, 431 MB, 84 us, 5.1 TB/s; one sequence of 500
 // 8.8 us, a chain of loads.  Two to four tiles of rows a wave, loads a group ahead and pairs of waves that share a group's dims were no faster.
 #pragma once
