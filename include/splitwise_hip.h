@@ -424,7 +424,7 @@ int sw_context_attention_split(void* out, const void* query, const void* key, co
 
 /* ------------------------------------------- an 8-bit cache with a scale for each (block, kv head)
  * No counterpart in the reference, whose 8-bit cache is unscaled e5m2.  Codes are one byte, int8 in -127 .. 127
- * (SW_I8_SCALED) or e4m3 (SW_E4M3_SCALED), and stand for code * scale:
+ * (SW_I8_SCALED) or e4m3 (SW_E4M3_SCALED), and stand for code * scale, where no scale is below 0:
  *   key_cache      [num_blocks, kv_heads, head_size/16, block_size, 16]       key_scales    fp32 [num_blocks, kv_heads]
  *   value_cache    [num_blocks, kv_heads, head_size, block_size]              value_scales  fp32 [num_blocks, kv_heads]
  * all contiguous, the caches on 16 bytes.  head_size 64, 80, 96, 112, 128 or 256, block_size 8, 16 or 32.  A block table's

@@ -12,7 +12,7 @@
 //     exp2, one addition, half a maximum and half a packing;
 //   * sums are rescaled only where a row's maximum or its reference may have grown by more than 2^8: the largest score and the largest
 //     value scale of a stage say so, and only then is looked for the largest of both together.
-// Measured: 2041 tokens of 64 heads of 128 on 8 behind 14003, bf16, int8, 1001 to 1027 us by box (under a profiler 1071 to 1203), 1.0
+// Measured: 2041 tokens of 64 heads of 128 on 8 behind 14003, bf16, int8, 1001 to 1027 us from card to card (under a profiler 1071 to 1203), 1.0
 // PFLOP/s, where a plain product of large matrices reaches 1.2: matrix cores busy 47 % of the cycles and vector units 57 %, at a clock that
 // the power lets down to 2 GHz.  (So what takes vector instructions out counts, not what moves them: two halves of the waves half a stage
 // apart, with a barrier more, 1135; all products of a stage together and its weights behind them 1125.)  8 x 1024 of 32 heads on 8 behind
