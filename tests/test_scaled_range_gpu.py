@@ -261,3 +261,22 @@ def test_windows_wider_than_any_context(kind, window, heads):
     assert torch.equal(got, context(c, query, tables, [0, 70], new, lens, 0.1))
     assert (got[:30] == 0).all()
     check(got, c, query, tables, lens, new, 0.1)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size,block,heads,kv_heads", SHAPES)
+@pytest.mark.parametrize("parts", [1, 3, None])
+def test_attention_repeats_itself(kind, size, block, heads, kv_heads, parts):
+    """The same bits from the same call, of few and of many rows, whatever the workspace held."""
+    new, lens = [200, 5], [900, 330]
+    c = Cache(sum((n + block - 1) // block for n in lens) + 1, kv_heads, size, block, kind)
+    tables = tables_for(lens, block, c.key.shape[0])
+    query = random_query(205, heads, size, torch.float16)
+    few = [5, 5]
+    first = [context(c, query, tables, [0, 200], new, lens, 0.09, parts), context(c, query, tables, [0, 5], few, lens, 0.09, parts),
+             decode(c, query[:2], tables, lens, 0.09, parts=parts)]
+    for _ in range(4):
+        torch.empty(1 << 22, device=DEV).fill_(math.nan)
+        again = [context(c, query, tables, [0, 200], new, lens, 0.09, parts), context(c, query, tables, [0, 5], few, lens, 0.09, parts),
+                 decode(c, query[:2], tables, lens, 0.09, parts=parts)]
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
